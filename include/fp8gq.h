@@ -543,6 +543,107 @@ int fp8gq_gemv_quant_tm_noalloc(const void *x, int64_t ldx, const void *w, int64
                                 int M, int N, int K, uint8_t *xq_out, float *sx_out,
                                 fp8gq_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Serving operators: what a decode or prompt step runs between the qkv and o
+ * linears, and after the lm_head.  Element type codes: */
+#define FP8GQ_DTYPE_BF16 0
+#define FP8GQ_DTYPE_E4M3 1
+#define FP8GQ_DTYPE_F32 2
+
+/* A paged key-value cache: `num_pages` pages of `page_size` token slots, each
+ * slot holding Hkv heads of D values of k and of v (dtype BF16, or E4M3 whose
+ * values stand for value * k_scale / value * v_scale).  Strides are in
+ * elements; the D values of a head are contiguous.  k, v and every stride are
+ * multiples of 16 bytes. */
+typedef struct fp8gq_paged_cache {
+    void *k, *v;
+    int64_t k_page_stride, k_slot_stride, k_head_stride;
+    int64_t v_page_stride, v_slot_stride, v_head_stride;
+    int64_t num_pages;
+    int page_size;
+    int dtype;
+    float k_scale, v_scale;
+} fp8gq_paged_cache;
+
+/* Per-head RMS norm and rotary positions of q and k, and the write of k and v
+ * into the paged cache, for T tokens:
+ *   qkv      bf16 [T, (Hq + 2 Hkv) * D], row stride ldqkv: q heads, k heads, v heads
+ *   norm     n(x) = x / sqrt(mean(x^2) + eps) * w for q (q_weight bf16 [D]) and
+ *            k (k_weight); NULL: no norm
+ *   rotary   cos_sin fp32 [max_position, D]: D/2 cosines, then D/2 sines;
+ *            (a, b) = the halves of a head -> (a cos - b sin, b cos + a sin)
+ *   positions, slots  int64 [T]; slot = page * page_size + place in the page,
+ *            negative: the token is not stored (padding)
+ *   q_out    bf16 [T, Hq, D], token stride ldq (may be qkv itself)
+ *   k_out    bf16 [T, Hkv, D], token stride ldk, or NULL: k as it is before the cache's rounding
+ * Computed in fp32 and rounded once.  D is 64 or 128.  T == 0 does nothing.
+ * A position or slot past its range is recorded in the device error word; the
+ * token's position is clamped, its k and v are not stored.
+ * The reference's qk_norm_rope_kernel (kernels/fused_qk_rope.py:16-41) has
+ * the norm and the rotation; it has no cache. */
+int fp8gq_qk_norm_rope_append(const void *qkv, int64_t ldqkv, const int64_t *positions,
+                              const int64_t *slots, const float *cos_sin, int64_t max_position,
+                              const void *q_weight, const void *k_weight, float eps,
+                              void *q_out, int64_t ldq, void *k_out, int64_t ldk,
+                              const fp8gq_paged_cache *cache, int T, int Hq, int Hkv, int D,
+                              fp8gq_stream_t stream);
+
+/* Attention of one new token per sequence over the paged cache:
+ *   out[b, h] = sum_j softmax_j(scale * q[b, h] . k[j, h / (Hq / Hkv)]) v[j, ...], j < lens[b]
+ *   q, out      bf16 [B, Hq, D], token and head strides in elements (multiples of 8)
+ *   page_table  int32 [B, max_pages], row stride ld_table: the pages of a sequence in order
+ *   lens        int32 [B], the tokens a sequence has in the cache (the new one included)
+ *   lse         fp32 [B, Hq] or NULL: log of the softmax's sum
+ * A sequence of length 0 gives 0 (and lse -inf).  Scores, the softmax and the
+ * sums are fp32.  A length past max_pages * page_size is cut there, a page
+ * outside the cache counts as absent; both are recorded in the device error
+ * word.  Slots past a sequence's length may hold anything, NaN included.
+ * workspace as for the tile kernel: fp8gq_paged_decode_workspace_bytes bytes,
+ * zero-filled before its first use; may be shared with the tile kernel's
+ * calls of the same stream.  D is 64 or 128; Hq is a multiple of Hkv. */
+size_t fp8gq_paged_decode_workspace_bytes(int Hq, int Hkv, int D);
+int fp8gq_paged_decode_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                                 const fp8gq_paged_cache *cache, const int32_t *page_table,
+                                 int64_t ld_table, int max_pages, const int32_t *lens,
+                                 void *out, int64_t o_token_stride, int64_t o_head_stride, float *lse,
+                                 int B, int Hq, int Hkv, int D, float scale,
+                                 void *workspace, size_t workspace_bytes, fp8gq_stream_t stream);
+
+/* Attention over whole prompts, packed one after the other:
+ *   q, out  bf16 [Tq, Hq, D]; k, v bf16 [Tk, Hkv, D]; token and head strides in elements
+ *           (multiples of 8)
+ *   cu_q, cu_k  int32 [B + 1], ascending from 0: sequence b has the q tokens
+ *           cu_q[b] .. cu_q[b + 1] and the k tokens cu_k[b] .. cu_k[b + 1]
+ *   causal  row i of a sequence sees keys j <= i + (k tokens - q tokens): its
+ *           last row sees every key (a chunk of a prompt behind its prefix)
+ *   lse     fp32 [Tq, Hq] or NULL
+ * A row that sees no key gives 0 (and lse -inf).  Rows of out past cu_q[B] are
+ * not written.  Values of other sequences never reach a row, NaN included; a
+ * sequence's own k and v are taken to be finite (a masked v that is infinite
+ * or NaN may reach the rows of its tile).  An offset out of range is cut to
+ * [0, Tq] or [0, Tk] and recorded in the device error word. */
+int fp8gq_prompt_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                           const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                           const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                           void *out, int64_t o_token_stride, int64_t o_head_stride, float *lse,
+                           const int32_t *cu_q, const int32_t *cu_k, int B, int Tq, int Tk,
+                           int Hq, int Hkv, int D, float scale, int causal, fp8gq_stream_t stream);
+
+/* Log probabilities of given tokens under softmax(logits), with the entropy
+ * and the `top_k` likeliest tokens of each row:
+ *   logits  BF16 or F32 [T, V], row stride ld (any)
+ *   tokens  int64 [T]; a negative one (no token given) has logprob 0, one past
+ *           V has NaN and is recorded in the device error word
+ *   logprobs, entropy  fp32 [T] (nats); either may be NULL (tokens too, without logprobs)
+ *   top_ids int64 [T, top_k], top_logprobs fp32 [T, top_k]: descending, equal
+ *           logits by ascending index; 0 <= top_k <= min(32, V)
+ * A logit of -inf is a token ruled out.  A row with NaN or +inf, or without a
+ * finite logit, has NaN for every logprob and its entropy (its top_ids rank
+ * NaN above +inf).  Sums are fp32 over one pass. */
+int fp8gq_token_logprobs(const void *logits, int64_t ld, int dtype, const int64_t *tokens, int T, int V,
+                         float *logprobs, float *entropy, int64_t *top_ids, float *top_logprobs,
+                         int top_k, fp8gq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

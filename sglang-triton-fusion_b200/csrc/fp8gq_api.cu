@@ -15,6 +15,7 @@
 
 #include "../../include/fp8gq.h"
 #include "fp8gq_device.cuh"
+#include "host_common.h"
 #include "gemm_tm.cuh"
 #include "gemv_row.cuh"
 #include "quant_only.cuh"
@@ -27,18 +28,9 @@ using namespace fp8gq;
 
 namespace {
 
-constexpr int kMaxDevices = 64;
 constexpr uint64_t kMinWaitLimitNs = 1000000ull;        // 1 ms
 constexpr uint64_t kMaxWaitLimitNs = 20000000000ull;    // 20 s
 
-struct DeviceInfo {
-  int sm_count = 0;
-  int cc_major = 0;
-  int max_smem_optin = 0;
-};
-
-std::mutex g_mu;
-DeviceInfo g_dev[kMaxDevices];
 std::atomic<int> g_static_weights{0};
 std::atomic<int> g_tm_options{0};   // FP8GQ_TM_* bits
 
@@ -50,28 +42,6 @@ int tm_resident_mode() {
 }
 int tm_cluster_mode() { return (g_tm_options.load(std::memory_order_relaxed) & FP8GQ_TM_WORKSPACE_SPLITK) ? 0 : 1; }
 
-int device_info(DeviceInfo* out, int* dev_out) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return FP8GQ_ERR_DEVICE;
-  std::lock_guard<std::mutex> lk(g_mu);
-  DeviceInfo& d = g_dev[dev];
-  if (d.sm_count == 0) {
-    if (cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&d.cc_major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&d.max_smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) !=
-            cudaSuccess) {
-      d.sm_count = 0;
-      return FP8GQ_ERR_DEVICE;
-    }
-  }
-  if (d.cc_major != 10) return FP8GQ_ERR_DEVICE;
-  *out = d;
-  if (dev_out) *dev_out = dev;
-  return FP8GQ_OK;
-}
-
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 int check_common(const void* x, const void* w, const float* ws, const void* out, int M, int N, int K,
                  int64_t ldw, int64_t ldws, int64_t ldo) {
   if (!x || !w || !ws || !out) return FP8GQ_ERR_NULL_POINTER;
@@ -81,18 +51,6 @@ int check_common(const void* x, const void* w, const float* ws, const void* out,
   if ((reinterpret_cast<uintptr_t>(ws) & 3u) != 0 || (reinterpret_cast<uintptr_t>(out) & 1u) != 0)
     return FP8GQ_ERR_ALIGNMENT;
   return FP8GQ_OK;
-}
-
-// FP8GQ_ERR_LAUNCH for a failed CUDA call; with FP8GQ_DEBUG set in the
-// environment the CUDA error is also printed to stderr.
-int cuda_fail(cudaError_t e, const char* what) {
-  static const bool debug = std::getenv("FP8GQ_DEBUG") != nullptr;
-  if (debug) std::fprintf(stderr, "fp8gq: %s: %s\n", what, cudaGetErrorString(e));
-  return FP8GQ_ERR_LAUNCH;
-}
-
-inline int launch_status() {
-  return cudaGetLastError() == cudaSuccess ? FP8GQ_OK : FP8GQ_ERR_LAUNCH;
 }
 
 // ----------------------------------------------------------------- row --
@@ -726,6 +684,7 @@ int fp8gq_set_wait_limit_ns(uint64_t limit_ns, uint64_t* previous) {
   if (cudaMemcpyFromSymbol(&old, g_wait_limit_ns, sizeof(old)) != cudaSuccess) return FP8GQ_ERR_LAUNCH;
   const unsigned long long v = limit_ns;
   if (cudaMemcpyToSymbol(g_wait_limit_ns, &v, sizeof(v)) != cudaSuccess) return FP8GQ_ERR_LAUNCH;
+  if (serve_set_wait_limit(v) != FP8GQ_OK) return FP8GQ_ERR_LAUNCH;
   if (previous) *previous = old;
   return FP8GQ_OK;
 }
@@ -739,6 +698,9 @@ int fp8gq_device_error(uint32_t* code, int clear) {
     const unsigned int zero = 0;
     if (cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero)) != cudaSuccess) return FP8GQ_ERR_LAUNCH;
   }
+  unsigned int serve = 0;
+  if (serve_error_word(&serve, clear) != FP8GQ_OK) return FP8GQ_ERR_LAUNCH;
+  if (!*code) *code = serve;   // both set: the linears' is reported (a lost peer)
   return FP8GQ_OK;
 }
 

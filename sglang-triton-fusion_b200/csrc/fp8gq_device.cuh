@@ -20,8 +20,9 @@ constexpr float kE4m3Max = 448.0f;   // largest finite e4m3fn value
 constexpr float kEps = 1e-10f;       // amax floor (kernels/fused_gemv_quant_tm.py:144)
 
 // Error word written when a bounded wait gives up (read by fp8gq_device_error).
-// Low 16 bits: site id; bit 31: set.  libfp8gq is one translation unit
-// (fp8gq_api.cu), which is where this definition lands.
+// Low 16 bits: site id; bit 31: set.  Each translation unit has its own (the
+// linears' in fp8gq_api.cu, the serving operators' in serve_api.cu);
+// fp8gq_device_error reads them all.
 __device__ unsigned int g_device_error = 0;
 
 enum ErrorSite : unsigned int {
@@ -35,6 +36,8 @@ enum ErrorSite : unsigned int {
   kSiteGather = 8,       // waiting for the peers' output slices of a gathered linear
   kSiteStackRing = 9,    // stack runner: a ring, accumulator or scale wait inside a CTA
   kSiteStackDep = 10,    // stack runner: waiting for every CTA to finish an earlier linear
+  kSitePrompt = 11,      // prompt attention: a ring, score or accumulator wait inside a CTA
+  kSiteBadIndex = 12,    // a serving operator met a position, slot, page, length, offset or token out of range
 };
 
 __device__ __forceinline__ void record_error(unsigned int site) {

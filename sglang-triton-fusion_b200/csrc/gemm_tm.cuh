@@ -60,6 +60,8 @@
 #include <tuple>
 
 #include "fp8gq_device.cuh"
+#include "host_common.h"
+#include "tensor_core.cuh"
 #include "quant_only.cuh"
 
 namespace fp8gq {
@@ -169,42 +171,6 @@ __device__ __forceinline__ uint64_t l2_policy_evict_last() {
   return pol;
 }
 
-// Fetch a tensor map (a __grid_constant__ kernel parameter) into the TMA
-// descriptor cache ahead of its first use.
-__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-
-// Cluster-wide barrier: every thread of every CTA of the cluster arrives; the
-// release/acquire pair orders shared-memory writes before it with
-// distributed-shared-memory reads after it.
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// Shared-memory address of the same variable in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t dsmem_addr(const void* local, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float ld_dsmem(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
 // K-major operand in the 128-byte swizzle layout: 8-row atoms of 1024 bytes
 // stacked at SBO = 1024; version 1 (tcgen05); layout type 2 (SWIZZLE_128B).
 __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
@@ -233,12 +199,6 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t
       : "memory");
 }
 
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-}
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   uint32_t r[16];
   asm volatile(
@@ -264,12 +224,6 @@ __device__ __forceinline__ bool tag_wait(volatile uint32_t* tag, uint32_t want) 
       return false;
     }
   }
-}
-
-__device__ __forceinline__ int atomic_add_acq_rel_gpu(int* addr, int v) {
-  int old;
-  asm volatile("atom.add.acq_rel.gpu.s32 %0, [%1], %2;" : "=r"(old) : "l"(addr), "r"(v) : "memory");
-  return old;
 }
 
 // Walks a CTA's tiles in order with no integer division on the way (the
@@ -1287,19 +1241,6 @@ inline size_t tm_workspace_bytes(int M, int N, int K) {
   return tm_workspace_bytes_for(M, N, K, sms);
 }
 
-inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static std::once_flag once;
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  });
-  return fn;
-}
-
 // Weight tensor map: 2-D uint8 [N rows, K bytes] with row stride ldw, box
 // 128 x 128 bytes, 128-byte swizzle (the UMMA K-major SW128 layout).
 inline bool make_weight_tmap(CUtensorMap* map, const void* w, int N, int K, int64_t ldw) {
@@ -1385,27 +1326,6 @@ inline bool cached_tmap(CUtensorMap* map, int kind, const void* ptr, int rows, i
   if (cache.size() >= kTmapCacheMax) cache.clear();
   cache.emplace(key, *map);
   return true;
-}
-
-// cudaFuncAttributeMaxDynamicSharedMemorySize raised to the device's limit
-// once per kernel and device (launches then pass their own smaller sizes).
-inline cudaError_t ensure_max_smem(const void* fn, int max_smem) {
-  static std::mutex mu;
-  static std::map<std::pair<int, const void*>, int> done;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const auto key = std::make_pair(dev, fn);
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = done.find(key);
-    if (it != done.end() && it->second >= max_smem) return cudaSuccess;
-  }
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lock(mu);
-  done[key] = max_smem;
-  return cudaSuccess;
 }
 
 // cudaFuncAttributeNonPortableClusterSizeAllowed set once per kernel and

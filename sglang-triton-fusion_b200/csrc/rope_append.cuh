@@ -1,0 +1,164 @@
+// Per-head RMS norm + rotary positions of q and k, and the write of k and v
+// into a paged cache (bf16, or e4m3 of value / scale).
+//
+// HBM-bound streaming: every value is read once and written once.  D / 16
+// lanes own one head of one token; a lane holds 8 values of the head's first
+// half and the 8 values they rotate with in the second half (two 16-byte
+// loads), so the rotation needs no exchange and the norm's sum of squares a
+// butterfly over D / 16 lanes.  fp32 throughout, one rounding at the store.
+#pragma once
+
+#include "fp8gq_device.cuh"
+
+namespace fp8gq {
+
+// A paged cache as the kernels see it (strides in elements).
+struct CacheView {
+  void* k;
+  void* v;
+  int64_t k_page, k_slot, k_head;
+  int64_t v_page, v_slot, v_head;
+  int64_t num_pages;
+  int page_size;
+  float k_scale, v_scale;
+};
+
+struct AppendParams {
+  const __nv_bfloat16* qkv;
+  int64_t ldqkv;
+  const int64_t* positions;
+  const int64_t* slots;
+  const float* cos_sin;
+  int64_t max_position;
+  const __nv_bfloat16* qw;
+  const __nv_bfloat16* kw;
+  float eps;
+  __nv_bfloat16* q_out;
+  int64_t ldq;
+  __nv_bfloat16* k_out;
+  int64_t ldk;
+  CacheView cache;
+  int T, Hq, Hkv;
+};
+
+constexpr int kAppendThreads = 256;
+
+__device__ __forceinline__ void unpack8(float (&v)[8], uint4 a) {
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[2 * e] = bf16_lo(w[e]);
+    v[2 * e + 1] = bf16_hi(w[e]);
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+    w[e] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 8 values -> 8 e4m3 codes of value / scale (IEEE division, saturating).
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], float scale) {
+  uint32_t h[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    h[e] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[2 * e], scale), __fdiv_rn(v[2 * e + 1], scale)),
+                                    __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+template <int D, bool kFp8>
+__global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const AppendParams p) {
+  constexpr int L = D / 16;              // lanes per head
+  grid_dependency_wait();
+  const int heads = p.Hq + 2 * p.Hkv;
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x) / L;
+  const int l = threadIdx.x % L;
+  const bool live = unit < static_cast<int64_t>(p.T) * heads;
+  // lanes past the end follow the last unit through the shuffles and store nothing
+  const int64_t u = live ? unit : static_cast<int64_t>(p.T) * heads - 1;
+  const int64_t t = u / heads;
+  const int h = static_cast<int>(u - t * heads);
+  const __nv_bfloat16* src = p.qkv + t * p.ldqkv + static_cast<int64_t>(h) * D + 8 * l;
+  float a[8], b[8];
+  unpack8(a, *reinterpret_cast<const uint4*>(src));
+  unpack8(b, *reinterpret_cast<const uint4*>(src + D / 2));
+  const bool is_q = h < p.Hq;
+  const bool is_v = h >= p.Hq + p.Hkv;
+  const __nv_bfloat16* w = is_v ? nullptr : is_q ? p.qw : p.kw;
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (w) {
+    const float rstd = 1.0f / sqrtf(ss / D + p.eps);
+    float wa[8], wb[8];
+    unpack8(wa, *reinterpret_cast<const uint4*>(w + 8 * l));
+    unpack8(wb, *reinterpret_cast<const uint4*>(w + D / 2 + 8 * l));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      a[e] = a[e] * rstd * wa[e];
+      b[e] = b[e] * rstd * wb[e];
+    }
+  }
+  if (!is_v) {
+    int64_t pos = p.positions[t];
+    if (pos < 0 || pos >= p.max_position) {
+      record_error(kSiteBadIndex);
+      pos = pos < 0 ? 0 : p.max_position - 1;
+    }
+    const float4* c = reinterpret_cast<const float4*>(p.cos_sin + pos * D + 8 * l);
+    const float4* s = reinterpret_cast<const float4*>(p.cos_sin + pos * D + D / 2 + 8 * l);
+    const float4 c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
+    const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = a[e] * cs[e] - b[e] * sn[e];
+      b[e] = b[e] * cs[e] + a[e] * sn[e];
+      a[e] = x;
+    }
+  }
+  if (live) {
+    if (is_q) {
+      __nv_bfloat16* o = p.q_out + t * p.ldq + static_cast<int64_t>(h) * D + 8 * l;
+      *reinterpret_cast<uint4*>(o) = pack8(a);
+      *reinterpret_cast<uint4*>(o + D / 2) = pack8(b);
+    } else {
+      const int hk = (h - p.Hq) % p.Hkv;
+      if (!is_v && p.k_out) {
+        __nv_bfloat16* o = p.k_out + t * p.ldk + static_cast<int64_t>(hk) * D + 8 * l;
+        *reinterpret_cast<uint4*>(o) = pack8(a);
+        *reinterpret_cast<uint4*>(o + D / 2) = pack8(b);
+      }
+      const int64_t slot = p.slots[t];
+      if (slot >= p.cache.num_pages * p.cache.page_size) {
+        record_error(kSiteBadIndex);
+      } else if (slot >= 0) {
+        const int64_t page = slot / p.cache.page_size;
+        const int64_t at = slot - page * p.cache.page_size;
+        const int64_t off = (is_v ? page * p.cache.v_page + at * p.cache.v_slot + hk * p.cache.v_head
+                                  : page * p.cache.k_page + at * p.cache.k_slot + hk * p.cache.k_head) + 8 * l;
+        if constexpr (kFp8) {
+          const float scale = is_v ? p.cache.v_scale : p.cache.k_scale;
+          uint8_t* o = static_cast<uint8_t*>(is_v ? p.cache.v : p.cache.k) + off;
+          *reinterpret_cast<uint2*>(o) = quant8(a, scale);
+          *reinterpret_cast<uint2*>(o + D / 2) = quant8(b, scale);
+        } else {
+          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(is_v ? p.cache.v : p.cache.k) + off;
+          *reinterpret_cast<uint4*>(o) = pack8(a);
+          *reinterpret_cast<uint4*>(o + D / 2) = pack8(b);
+        }
+      }
+    }
+  }
+  grid_launch_dependents();
+}
+
+}  // namespace fp8gq

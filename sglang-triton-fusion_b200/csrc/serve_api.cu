@@ -1,0 +1,264 @@
+// C ABI of the serving operators (declared in include/fp8gq.h): argument
+// checks, kernel selection and launch.
+#include <cuda_runtime.h>
+
+#include "../../include/fp8gq.h"
+#include "fp8gq_device.cuh"
+#include "host_common.h"
+#include "paged_decode.cuh"
+#include "prompt_attention.cuh"
+#include "rope_append.cuh"
+#include "token_logprobs.cuh"
+
+namespace fp8gq {
+
+int serve_error_word(unsigned int* code, int clear) {
+  if (cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code)) != cudaSuccess) return FP8GQ_ERR_LAUNCH;
+  if (clear && *code) {
+    const unsigned int zero = 0;
+    if (cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero)) != cudaSuccess) return FP8GQ_ERR_LAUNCH;
+  }
+  return FP8GQ_OK;
+}
+
+int serve_set_wait_limit(unsigned long long limit_ns) {
+  return cudaMemcpyToSymbol(g_wait_limit_ns, &limit_ns, sizeof(limit_ns)) == cudaSuccess ? FP8GQ_OK : FP8GQ_ERR_LAUNCH;
+}
+
+}  // namespace fp8gq
+
+using namespace fp8gq;
+
+namespace {
+
+int check_heads(int Hq, int Hkv, int D) {
+  if (Hq < 1 || Hkv < 1 || Hq % Hkv) return FP8GQ_ERR_SHAPE;
+  if (D != 64 && D != 128) return FP8GQ_ERR_UNSUPPORTED;
+  return FP8GQ_OK;
+}
+
+// A cache's checks; strides are multiples of 16 bytes and (for a cache with
+// several pages, slots or heads) positive.
+int to_cache_view(const fp8gq_paged_cache* c, int Hkv, int D, CacheView* v) {
+  if (!c || !c->k || !c->v) return FP8GQ_ERR_NULL_POINTER;
+  if (c->num_pages < 1 || c->page_size < 1 || c->num_pages > INT32_MAX) return FP8GQ_ERR_SHAPE;
+  if (c->dtype != FP8GQ_DTYPE_BF16 && c->dtype != FP8GQ_DTYPE_E4M3) return FP8GQ_ERR_UNSUPPORTED;
+  const int64_t st[6] = {c->k_page_stride, c->k_slot_stride, c->k_head_stride,
+                         c->v_page_stride, c->v_slot_stride, c->v_head_stride};
+  const int64_t n[3] = {c->num_pages, c->page_size, Hkv};
+  const int unit = c->dtype == FP8GQ_DTYPE_BF16 ? 8 : 16;
+  for (int i = 0; i < 6; ++i) {
+    if (n[i % 3] > 1 && st[i] < D) return FP8GQ_ERR_STRIDE;
+    if (st[i] % unit) return FP8GQ_ERR_ALIGNMENT;
+  }
+  if (!aligned16(c->k) || !aligned16(c->v)) return FP8GQ_ERR_ALIGNMENT;
+  if (c->dtype == FP8GQ_DTYPE_E4M3 && !(c->k_scale > 0.0f && c->v_scale > 0.0f)) return FP8GQ_ERR_UNSUPPORTED;
+  v->k = c->k;
+  v->v = c->v;
+  v->k_page = st[0];
+  v->k_slot = st[1];
+  v->k_head = st[2];
+  v->v_page = st[3];
+  v->v_slot = st[4];
+  v->v_head = st[5];
+  v->num_pages = c->num_pages;
+  v->page_size = c->page_size;
+  v->k_scale = c->k_scale;
+  v->v_scale = c->v_scale;
+  return FP8GQ_OK;
+}
+
+// q, k, v or out [tokens, heads, D] bf16: strides of at least a head, 16-byte
+// rows.
+int check_rows(const void* p, int64_t token, int64_t head, int tokens, int heads, int D) {
+  if (!p) return FP8GQ_ERR_NULL_POINTER;
+  if ((tokens > 1 && token < D) || (heads > 1 && head < D)) return FP8GQ_ERR_STRIDE;
+  if (!aligned16(p) || token % 8 || head % 8) return FP8GQ_ERR_ALIGNMENT;
+  return FP8GQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp8gq_qk_norm_rope_append(const void* qkv, int64_t ldqkv, const int64_t* positions, const int64_t* slots,
+                              const float* cos_sin, int64_t max_position, const void* q_weight, const void* k_weight,
+                              float eps, void* q_out, int64_t ldq, void* k_out, int64_t ldk,
+                              const fp8gq_paged_cache* cache, int T, int Hq, int Hkv, int D, fp8gq_stream_t stream) {
+  if (T < 0) return FP8GQ_ERR_SHAPE;
+  int st = check_heads(Hq, Hkv, D);
+  if (st != FP8GQ_OK) return st;
+  AppendParams p{};
+  st = to_cache_view(cache, Hkv, D, &p.cache);
+  if (st != FP8GQ_OK) return st;
+  if (T == 0) return FP8GQ_OK;
+  if (!qkv || !positions || !slots || !cos_sin || !q_out) return FP8GQ_ERR_NULL_POINTER;
+  const int64_t heads = static_cast<int64_t>(Hq) + 2 * static_cast<int64_t>(Hkv);
+  if (max_position < 1 || heads > INT32_MAX / D) return FP8GQ_ERR_SHAPE;
+  if (T > 1 && (ldqkv < heads * D || ldq < static_cast<int64_t>(Hq) * D ||
+                (k_out && ldk < static_cast<int64_t>(Hkv) * D)))
+    return FP8GQ_ERR_STRIDE;
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(cos_sin) || !aligned16(q_weight) ||
+      !aligned16(k_weight) || ldqkv % 8 || ldq % 8 || (k_out && ldk % 8))
+    return FP8GQ_ERR_ALIGNMENT;
+  DeviceInfo di;
+  st = device_info(&di, nullptr);
+  if (st != FP8GQ_OK) return st;
+  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  p.ldqkv = ldqkv;
+  p.positions = positions;
+  p.slots = slots;
+  p.cos_sin = cos_sin;
+  p.max_position = max_position;
+  p.qw = static_cast<const __nv_bfloat16*>(q_weight);
+  p.kw = static_cast<const __nv_bfloat16*>(k_weight);
+  p.eps = eps;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.ldq = ldq;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.ldk = ldk;
+  p.T = T;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  const int64_t threads = static_cast<int64_t>(T) * heads * (D / 16);
+  const int64_t blocks = (threads + kAppendThreads - 1) / kAppendThreads;
+  if (blocks > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
+  const bool fp8 = cache->dtype == FP8GQ_DTYPE_E4M3;
+  auto fn = D == 128 ? (fp8 ? rope_append_kernel<128, true> : rope_append_kernel<128, false>)
+                     : (fp8 ? rope_append_kernel<64, true> : rope_append_kernel<64, false>);
+  const cudaError_t e = launch_with_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0,
+                                        static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_qk_norm_rope_append");
+}
+
+size_t fp8gq_paged_decode_workspace_bytes(int Hq, int Hkv, int D) {
+  (void)Hq;
+  (void)Hkv;
+  (void)D;
+  return 0;
+}
+
+int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                 const fp8gq_paged_cache* cache, const int32_t* page_table, int64_t ld_table,
+                                 int max_pages, const int32_t* lens, void* out, int64_t o_token_stride,
+                                 int64_t o_head_stride, float* lse, int B, int Hq, int Hkv, int D, float scale,
+                                 void* workspace, size_t workspace_bytes, fp8gq_stream_t stream) {
+  if (B < 0 || max_pages < 0) return FP8GQ_ERR_SHAPE;
+  int st = check_heads(Hq, Hkv, D);
+  if (st != FP8GQ_OK) return st;
+  DecodeParams p{};
+  st = to_cache_view(cache, Hkv, D, &p.cache);
+  if (st != FP8GQ_OK) return st;
+  if (B == 0) return FP8GQ_OK;
+  if (!lens || (!page_table && max_pages > 0)) return FP8GQ_ERR_NULL_POINTER;
+  st = check_rows(q, q_token_stride, q_head_stride, B, Hq, D);
+  if (st != FP8GQ_OK) return st;
+  st = check_rows(out, o_token_stride, o_head_stride, B, Hq, D);
+  if (st != FP8GQ_OK) return st;
+  if (B > 1 && ld_table < max_pages) return FP8GQ_ERR_STRIDE;
+  DeviceInfo di;
+  st = device_info(&di, nullptr);
+  if (st != FP8GQ_OK) return st;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_token = q_token_stride;
+  p.q_head = q_head_stride;
+  p.table = page_table;
+  p.ld_table = ld_table;
+  p.max_pages = max_pages;
+  p.lens = lens;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.o_token = o_token_stride;
+  p.o_head = o_head_stride;
+  p.lse = lse;
+  p.B = B;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.scale = scale;
+  const int64_t blocks = (static_cast<int64_t>(B) * Hq + 3) / 4;
+  if (blocks > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
+  const bool fp8 = cache->dtype == FP8GQ_DTYPE_E4M3;
+  auto fn = D == 128 ? (fp8 ? paged_decode_kernel<128, true> : paged_decode_kernel<128, false>)
+                     : (fp8 ? paged_decode_kernel<64, true> : paged_decode_kernel<64, false>);
+  const cudaError_t e = launch_with_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(128), 0,
+                                        static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_paged_decode_attention");
+}
+
+int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                           int64_t v_head_stride, void* out, int64_t o_token_stride, int64_t o_head_stride, float* lse,
+                           const int32_t* cu_q, const int32_t* cu_k, int B, int Tq, int Tk, int Hq, int Hkv, int D,
+                           float scale, int causal, fp8gq_stream_t stream) {
+  if (B < 0 || Tq < 0 || Tk < 0) return FP8GQ_ERR_SHAPE;
+  int st = check_heads(Hq, Hkv, D);
+  if (st != FP8GQ_OK) return st;
+  if (B == 0 || Tq == 0) return FP8GQ_OK;
+  if (!cu_q || !cu_k) return FP8GQ_ERR_NULL_POINTER;
+  st = check_rows(q, q_token_stride, q_head_stride, Tq, Hq, D);
+  if (st == FP8GQ_OK) st = check_rows(out, o_token_stride, o_head_stride, Tq, Hq, D);
+  if (st == FP8GQ_OK && Tk > 0) st = check_rows(k, k_token_stride, k_head_stride, Tk, Hkv, D);
+  if (st == FP8GQ_OK && Tk > 0) st = check_rows(v, v_token_stride, v_head_stride, Tk, Hkv, D);
+  if (st != FP8GQ_OK) return st;
+  DeviceInfo di;
+  st = device_info(&di, nullptr);
+  if (st != FP8GQ_OK) return st;
+  PromptParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.q_token = q_token_stride;
+  p.q_head = q_head_stride;
+  p.k_token = k_token_stride;
+  p.k_head = k_head_stride;
+  p.v_token = v_token_stride;
+  p.v_head = v_head_stride;
+  p.o_token = o_token_stride;
+  p.o_head = o_head_stride;
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.B = B;
+  p.Tq = Tq;
+  p.Tk = Tk;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.scale = scale;
+  p.causal = causal ? 1 : 0;
+  const int64_t blocks = (static_cast<int64_t>(Tq) * Hq + 3) / 4;
+  if (blocks > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
+  auto fn = D == 128 ? prompt_attention_kernel<128> : prompt_attention_kernel<64>;
+  const cudaError_t e = launch_with_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(128), 0,
+                                        static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_prompt_attention");
+}
+
+int fp8gq_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_t* tokens, int T, int V,
+                         float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs, int top_k,
+                         fp8gq_stream_t stream) {
+  if (T < 0 || V < 1 || top_k < 0 || top_k > V) return FP8GQ_ERR_SHAPE;
+  if (top_k > kMaxTop || (dtype != FP8GQ_DTYPE_BF16 && dtype != FP8GQ_DTYPE_F32)) return FP8GQ_ERR_UNSUPPORTED;
+  if (T == 0) return FP8GQ_OK;
+  if (!logits || (logprobs && !tokens) || (top_k > 0 && (!top_ids || !top_logprobs))) return FP8GQ_ERR_NULL_POINTER;
+  if (T > 1 && ld < V) return FP8GQ_ERR_STRIDE;
+  if (reinterpret_cast<uintptr_t>(logits) & (dtype == FP8GQ_DTYPE_BF16 ? 1u : 3u)) return FP8GQ_ERR_ALIGNMENT;
+  DeviceInfo di;
+  int st = device_info(&di, nullptr);
+  if (st != FP8GQ_OK) return st;
+  LogprobParams p{};
+  p.logits = logits;
+  p.ld = ld;
+  p.tokens = tokens;
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.top_ids = top_ids;
+  p.top_logprobs = top_logprobs;
+  p.T = T;
+  p.V = V;
+  p.K = top_k;
+  auto fn = dtype == FP8GQ_DTYPE_BF16 ? token_logprobs_kernel<__nv_bfloat16> : token_logprobs_kernel<float>;
+  const cudaError_t e = launch_with_pdl(fn, dim3(T), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_token_logprobs");
+}
+
+}  // extern "C"

@@ -11,6 +11,10 @@ Entry points:
   fused_reduce_add_rmsnorm_gemv_quant(partials, r, w, Wq, Ws)          + the sum of K-sharded partials
   StackRunner([Linear(x, Wq, Ws, out, swiglu)...])   a list of linears in one persistent launch
   prepare_fused_gemv_quant(...), LaunchList(plans).run()   calls recorded once, launched with no host work
+  qk_norm_rope_append(qkv, ...)    per-head norm + rotary of q and k, k and v into a paged cache (bf16 / e4m3)
+  paged_decode_attention(q, ...)   attention of one new token per sequence over the paged cache
+  prompt_attention(q, k, v, ...)   attention over packed prompts, causal, grouped heads
+  token_logprobs(logits, tokens)   log probabilities of given tokens, entropy, top alternatives
   patch_fp8_fused_tail             the sglang linear wrappers and install()
 The C ABI is include/fp8gq.h (libfp8gq.so next to this file).
 """
@@ -23,6 +27,8 @@ from .ops import (GROUP, TM, ShapeError, add_rmsnorm, fused_add_rmsnorm_gemv_qua
                   swiglu_group_quant, workspace)
 from .prepared import (LaunchList, Plan, prepare_fused_add_rmsnorm_gemv_quant, prepare_fused_gemv_quant,  # noqa: F401
                        prepare_fused_swiglu_q_gemm)
+from .serve import (TokenLogprobs, paged_decode_attention, prompt_attention, qk_norm_rope_append,  # noqa: F401
+                    token_logprobs)
 from .stack import Linear, StackRunner  # noqa: F401
 from .chain import ChainRunner, Link  # noqa: F401
 

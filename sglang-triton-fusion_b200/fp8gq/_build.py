@@ -13,14 +13,17 @@ PKG_DIR = Path(__file__).resolve().parent
 SRC_DIR = PKG_DIR.parent / "csrc"
 REPO_DIR = PKG_DIR.parent.parent
 LIB_PATH = PKG_DIR / "libfp8gq.so"
-SOURCES = ["fp8gq_api.cu"]
-HEADERS = ["fp8gq_device.cuh", "gemv_row.cuh", "gemm_tm.cuh", "quant_only.cuh", "swiglu_writer.cuh", "chain.cuh",
-           "add_rmsnorm.cuh", "stack.cuh"]
+SOURCES = ["fp8gq_api.cu", "serve_api.cu"]
+HEADERS = {"fp8gq_api.cu": ["fp8gq_device.cuh", "host_common.h", "tensor_core.cuh", "gemv_row.cuh", "gemm_tm.cuh",
+                            "quant_only.cuh", "swiglu_writer.cuh", "chain.cuh", "add_rmsnorm.cuh", "stack.cuh"],
+           "serve_api.cu": ["fp8gq_device.cuh", "host_common.h", "tensor_core.cuh", "rope_append.cuh",
+                            "paged_decode.cuh", "prompt_attention.cuh", "token_logprobs.cuh"]}
+OBJ_DIR = PKG_DIR / "build"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
 
@@ -32,33 +35,48 @@ def nvcc_path() -> str:
     return cand
 
 
-def _inputs():
-    files = [SRC_DIR / s for s in SOURCES] + [SRC_DIR / h for h in HEADERS]
-    files.append(REPO_DIR / "include" / "fp8gq.h")
-    return files
+def _inputs(source: str):
+    return [SRC_DIR / source, *[SRC_DIR / h for h in HEADERS[source]], REPO_DIR / "include" / "fp8gq.h"]
+
+
+def _newer_than(target: Path, files) -> bool:
+    if not target.exists():
+        return False
+    t = target.stat().st_mtime
+    return all(f.stat().st_mtime <= t for f in files)
 
 
 def up_to_date() -> bool:
-    if not LIB_PATH.exists():
-        return False
-    t = LIB_PATH.stat().st_mtime
-    return all(f.stat().st_mtime <= t for f in _inputs())
+    return _newer_than(LIB_PATH, [f for s in SOURCES for f in _inputs(s)])
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
-    """Compile libfp8gq.so next to this file unless it is already current."""
+    """Compile libfp8gq.so next to this file unless it is already current: one
+    object per translation unit, in parallel, those that are current reused."""
     if not force and up_to_date():
         return LIB_PATH
-    cmd = [nvcc_path(), *NVCC_FLAGS, *(extra_flags or []),
-           "-I", str(REPO_DIR / "include"),
-           "-o", str(LIB_PATH) + ".tmp", *[str(SRC_DIR / s) for s in SOURCES]]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    OBJ_DIR.mkdir(exist_ok=True)
+    jobs = []
+    for s in SOURCES:
+        obj = OBJ_DIR / (Path(s).stem + ".o")
+        if force or extra_flags or not _newer_than(obj, _inputs(s)):
+            cmd = [nvcc_path(), *NVCC_FLAGS, *(extra_flags or []), "-I", str(REPO_DIR / "include"),
+                   "-c", "-o", str(obj) + ".tmp", str(SRC_DIR / s)]
+            if verbose:
+                print(" ".join(cmd), file=sys.stderr)
+            jobs.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    said = [(obj, p.communicate()[0], p.returncode) for obj, p in jobs]
+    for obj, text, rc in said:
+        if rc != 0:
+            raise RuntimeError(f"nvcc failed ({rc}):\n{text}")
+        if verbose and text:
+            print(text, file=sys.stderr)
+        os.replace(str(obj) + ".tmp", obj)
+    link = [nvcc_path(), *NVCC_FLAGS, "-shared", "-o", str(LIB_PATH) + ".tmp",
+            *[str(OBJ_DIR / (Path(s).stem + ".o")) for s in SOURCES]]
+    res = subprocess.run(link, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    if verbose and (res.stdout or res.stderr):
-        print(res.stdout + res.stderr, file=sys.stderr)
     os.replace(str(LIB_PATH) + ".tmp", LIB_PATH)
     return LIB_PATH
 

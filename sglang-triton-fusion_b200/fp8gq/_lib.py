@@ -62,6 +62,15 @@ class ChainPlan(ctypes.Structure):
                 ("seq", ctypes.c_void_p), ("reserved", ctypes.c_int64 * 4)]
 
 
+class PagedCache(ctypes.Structure):
+    """struct fp8gq_paged_cache (include/fp8gq.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_page_stride", ctypes.c_int64), ("k_slot_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v_page_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+                ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+
 class LaunchPlan(ctypes.Structure):
     """struct fp8gq_launch_plan (include/fp8gq.h): opaque, copyable bytes."""
     _fields_ = [("opaque", ctypes.c_uint64 * 512)]
@@ -91,6 +100,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
+_F = ctypes.c_float
 SIGNATURES = {
     "fp8gq_version": (_I, []),
     "fp8gq_status_string": (ctypes.c_char_p, [_I]),
@@ -131,6 +141,14 @@ SIGNATURES = {
                                  ctypes.POINTER(ChainPlan)]),
     "fp8gq_chain_run": (_I, [ctypes.POINTER(ChainPlan), _P]),
     "fp8gq_gemv_quant_tm_noalloc": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P]),
+    "fp8gq_qk_norm_rope_append": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _P, _F, _P, _I64, _P, _I64,
+                                       ctypes.POINTER(PagedCache), _I, _I, _I, _I, _P]),
+    "fp8gq_paged_decode_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "fp8gq_paged_decode_attention": (_I, [_P, _I64, _I64, ctypes.POINTER(PagedCache), _P, _I64, _I, _P, _P, _I64, _I64,
+                                          _P, _I, _I, _I, _I, _F, _P, _SZ, _P]),
+    "fp8gq_prompt_attention": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P,
+                                    _I, _I, _I, _I, _I, _I, _F, _I, _P]),
+    "fp8gq_token_logprobs": (_I, [_P, _I64, _I, _P, _I, _I, _P, _P, _P, _P, _I, _P]),
     "fp8gq_prepare_fused_gemv_quant": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _SZ,
                                             ctypes.POINTER(LaunchPlan)]),
     "fp8gq_prepare_fused_swiglu_q_gemm": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _SZ,
