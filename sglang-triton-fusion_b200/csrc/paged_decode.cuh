@@ -1,11 +1,30 @@
 // Attention of one new token per sequence over a paged key-value cache.
 //
-// One warp per (sequence, query head): the lanes split the head's values, the
-// running maximum and sum of the softmax are kept over one pass.
+// Mathematics: o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q.k_j,
+// in one pass over the cache with the running maximum m; partial results
+// (m, l, o) of disjoint token ranges join by rescaling to the larger maximum.
+//
+// Bound: HBM, every cached byte read once (16 flops per byte at most, with the
+// heads padded to the matrix instruction's 8 columns).
+//
+// Work split: the tiles (4 warps x kTok tokens of one sequence and kv head) of
+// all sequences form one flat list, cut into equal contiguous ranges, one per
+// CTA, two CTAs per SM.  The lengths are read on the device (a captured step
+// replays while they grow), so ragged batches and long single sequences
+// balance the same way.  A (sequence, head) that lies in several ranges leaves
+// partial results in the workspace; the last CTA to arrive joins them in range
+// order, so the result does not depend on who is last.
+//
+// Inside a CTA each warp runs alone: it copies its own kTok rows of k and v
+// (8 KB per stage, 16-byte cp.async, kStages stages) and computes on them with
+// matrix instructions whose M side is the tokens (S^T = K Q^T, 16 x 8) and
+// then the head's values (O^T = V^T P^T), so a group of up to 8 query heads
+// wastes nothing of K and V and no barrier stands in the loop.
 #pragma once
 
 #include "fp8gq_device.cuh"
 #include "rope_append.cuh"
+#include "tensor_core.cuh"
 
 namespace fp8gq {
 
@@ -16,81 +35,647 @@ struct DecodeParams {
   const int32_t* table;
   int64_t ld_table;
   int max_pages;
+  int page_shift;           // log2(page_size), or -1
   const int32_t* lens;
   __nv_bfloat16* out;
   int64_t o_token, o_head;
   float* lse;
   int B, Hq, Hkv;
-  float scale;
+  int group;                // query heads per kv head
+  int blocks;               // head blocks (of 8 kNT query heads) per kv head
+  float scale_log2;         // softmax scale * log2(e) (* k_scale)
+  float out_scale;          // v_scale
+  int* counters;            // [grid], zero between launches
+  float* partials;          // [grid][2][kSlot]
 };
 
-template <int N>
-__device__ __forceinline__ float dot_warp(const float (&a)[N], const float (&b)[N]) {
-  float s = 0.0f;
-#pragma unroll
-  for (int e = 0; e < N; ++e) s += a[e] * b[e];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
-}
+constexpr int kDecWarps = 4;
+constexpr int kDecThreads = 32 * kDecWarps;
+constexpr int kDecStages = 3;
+constexpr int kDecStageBytes = 8192;        // k and v rows of one warp's step
+constexpr int kDecCounterBytes = 16384;     // the workspace's counters (the tile kernel's too)
+constexpr int kDecMinTiles = 2;             // tiles per CTA below which fewer CTAs work
 
 template <int D, bool kFp8>
-__global__ void __launch_bounds__(128) paged_decode_kernel(const DecodeParams p) {
-  constexpr int N = D / 32;
+struct DecCfg {
+  static constexpr int kRow = D * (kFp8 ? 1 : 2);       // bytes of a row
+  static constexpr int kTok = kDecStageBytes / 2 / kRow;
+  static constexpr int kTile = kTok * kDecWarps;
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kPad = D + 4;                    // o in shared memory: conflict-free fragment writes
+  static constexpr size_t kSmem = static_cast<size_t>(kDecWarps) * kDecStages * kDecStageBytes +
+                                  sizeof(float) * kDecWarps * 4 * kPad;
+};
+
+// Floats of one partial result: o [8 NT][D], m [8 NT], l [8 NT].
+inline __host__ __device__ constexpr int dec_slot_floats(int D, int NT) { return 8 * NT * (D + 2); }
+
+// Where 16-byte chunk c of row r lies: rows read by one phase of a shared-memory
+// load fall on different banks.
+template <int D, bool kFp8, bool kIsV>
+__device__ __forceinline__ uint32_t dec_chunk(int r, int c) {
+  constexpr int kRow = DecCfg<D, kFp8>::kRow;
+  if constexpr (!kFp8) return r * kRow + ((c ^ (r & 7)) << 4);
+  else if constexpr (D == 128) return r * kRow + ((kIsV ? c ^ (r & 6) : c ^ ((r & 1) << 2)) << 4);
+  else return r * kRow + ((kIsV ? c ^ ((r >> 1) & 3) : c) << 4);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// d += a (16 x 16) b (16 x 8), f16 or bf16 operands, fp32 sums.
+template <bool kF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kF16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// The length of sequence b, cut to what its page table can hold.
+__device__ __forceinline__ int dec_len(const DecodeParams& p, int b, bool record) {
+  const int64_t cap = static_cast<int64_t>(p.max_pages) * p.cache.page_size;
+  const int n = __ldg(p.lens + b);
+  if (n < 0 || n > cap) {
+    if (record) record_error(kSiteBadIndex);
+    return n < 0 ? 0 : static_cast<int>(cap);
+  }
+  return n;
+}
+
+// Four values of head h's output from their sum v and the weights' sum l
+// (relative to the maximum m); l = 0 where no token counted.
+template <int D>
+__device__ __forceinline__ void dec_store(const DecodeParams& p, int b, int h, int d, float4 v, float m, float l) {
+  const float r = l > 0.0f ? p.out_scale / l : l;      // NaN stays
+  uint2 w;
+  w.x = pack2<false>(v.x * r, v.y * r);
+  w.y = pack2<false>(v.z * r, v.w * r);
+  *reinterpret_cast<uint2*>(p.out + b * p.o_token + h * p.o_head + d) = w;
+  if (p.lse && d == 0)
+    p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// A place in the flat list of tiles.
+struct DecCursor {
+  int b, sub, j;       // sequence, (kv head, head block), tile of the sequence
+  int len, n;          // the sequence's tokens and tiles
+};
+
+template <int D, bool kFp8, int kNT>
+__global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const DecodeParams p) {
+  using Cfg = DecCfg<D, kFp8>;
+  constexpr int kTok = Cfg::kTok, kTile = Cfg::kTile, kMT = D / 16, kKT = D / 16, kTT = kTok / 16;
+  constexpr int kSlot = dec_slot_floats(D, kNT);
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t s_scan[kDecThreads];
+  __shared__ int64_t s_wsum[kDecWarps];
+  __shared__ uint64_t s_mask[kDecWarps][kDecStages];
+  __shared__ longlong2 s_off[kDecWarps][kTok];
+  __shared__ float s_m[kDecWarps][4], s_l[kDecWarps][4];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  unsigned char* ring = smem + warp * (kDecStages * kDecStageBytes);
+  const uint32_t ring_a = smem_u32(ring);
+  float* s_o = reinterpret_cast<float*>(smem + kDecWarps * kDecStages * kDecStageBytes);
+  const int items = p.Hkv * p.blocks;
+
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (w < static_cast<int64_t>(p.B) * p.Hq) {
-    const int b = static_cast<int>(w / p.Hq), h = static_cast<int>(w % p.Hq);
-    const int hk = h / (p.Hq / p.Hkv);
-    const int64_t cap = static_cast<int64_t>(p.max_pages) * p.cache.page_size;
-    int64_t n = p.lens[b];
-    if (n < 0 || n > cap) {
-      if (lane == 0) record_error(kSiteBadIndex);
-      n = n < 0 ? 0 : cap;
-    }
-    float q[N], acc[N];
+
+  // ---- the flat list: tiles of the sequences before each thread's share ----
+  const int share = (p.B + kDecThreads - 1) / kDecThreads;
+  const int b_lo = min(tid * share, p.B), b_hi = min(b_lo + share, p.B);
+  int64_t mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += (dec_len(p, b, blockIdx.x == 0) + kTile - 1) / kTile;
+  mine *= items;
+  int64_t incl = mine;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      q[e] = __bfloat162float(p.q[b * p.q_token + h * p.q_head + N * lane + e]) * p.scale *
-             (kFp8 ? p.cache.k_scale : 1.0f);
-      acc[e] = 0.0f;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) s_wsum[warp] = incl;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kDecWarps; ++w) {
+    if (w < warp) incl += s_wsum[w];
+    total += s_wsum[w];
+  }
+  s_scan[tid] = incl - mine;
+  __syncthreads();
+
+  // sequences without tokens
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    if (dec_len(p, b, false) > 0) continue;
+    for (int i = tid; i < p.Hq * (D / 8); i += kDecThreads)
+      *reinterpret_cast<uint4*>(p.out + b * p.o_token + (i / (D / 8)) * p.o_head + (i % (D / 8)) * 8) =
+          make_uint4(0, 0, 0, 0);
+    if (p.lse)
+      for (int h = tid; h < p.Hq; h += kDecThreads) p.lse[static_cast<int64_t>(b) * p.Hq + h] = -INFINITY;
+  }
+
+  const int64_t want = (total + kDecMinTiles - 1) / kDecMinTiles;
+  const int64_t ctas = want < gridDim.x ? want : gridDim.x;
+  const int64_t t0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : 0;
+  const int64_t t1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : 0;
+  if (t0 >= t1) {
+    grid_launch_dependents();
+    return;
+  }
+  auto owner = [&](int64_t t) { return ((t + 1) * ctas - 1) / total; };
+
+  // the tile t0: the thread share it falls in, then along that share
+  DecCursor cur;
+  int64_t item_t0;      // flat index of the current item's first tile
+  {
+    int lo = 0, hi = kDecThreads - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_scan[mid] <= t0) lo = mid;
+      else hi = mid - 1;
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t j = 0; j < n; ++j) {
-      const int64_t c = j / p.cache.page_size, at = j - c * p.cache.page_size;
-      const int64_t page = p.table[b * p.ld_table + c];
-      if (page < 0 || page >= p.cache.num_pages) {
-        if (lane == 0) record_error(kSiteBadIndex);
-        continue;
+    int64_t at = s_scan[lo];
+    int b = lo * share;
+    for (;; ++b) {
+      cur.len = dec_len(p, b, false);
+      cur.n = (cur.len + kTile - 1) / kTile;
+      const int64_t here = static_cast<int64_t>(cur.n) * items;
+      if (t0 < at + here) break;
+      at += here;
+    }
+    cur.b = b;
+    const int64_t in = t0 - at;
+    cur.sub = static_cast<int>(in / cur.n);
+    cur.j = static_cast<int>(in - static_cast<int64_t>(cur.sub) * cur.n);
+    item_t0 = t0 - cur.j;
+  }
+  auto next_item = [&](DecCursor& c) {
+    c.j = 0;
+    if (++c.sub == items) {
+      c.sub = 0;
+      do {
+        ++c.b;
+        c.len = dec_len(p, c.b, false);
+      } while (c.len == 0);
+      c.n = (c.len + kTile - 1) / kTile;
+    }
+  };
+
+  // ---- the copies of a step: page numbers one step ahead of the rows ----
+  constexpr int kIds = (kTok + 31) / 32;     // rows per lane whose pages it looks up
+  DecCursor pre = cur;                       // the next step to look up
+  int64_t pre_t = t0;
+  int id_page[kIds], id_at[kIds], id_head = 0;
+  bool id_ok[kIds];
+  auto look_up = [&]() {
+    if (pre_t >= t1) {
+#pragma unroll
+      for (int i = 0; i < kIds; ++i) id_ok[i] = false;
+      return;
+    }
+    id_head = pre.sub / p.blocks;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+      const int r = lane + 32 * i;
+      const int tok = pre.j * kTile + warp * kTok + r;
+      id_ok[i] = r < kTok && tok < pre.len;
+      if (id_ok[i]) {
+        const int c = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.cache.page_size;
+        id_at[i] = tok - c * p.cache.page_size;
+        id_page[i] = __ldg(p.table + pre.b * p.ld_table + c);
       }
-      const int64_t ko = page * p.cache.k_page + at * p.cache.k_slot + hk * p.cache.k_head + N * lane;
-      const int64_t vo = page * p.cache.v_page + at * p.cache.v_slot + hk * p.cache.v_head + N * lane;
-      float k[N], v[N];
+    }
+    ++pre_t;
+    if (++pre.j == pre.n && pre_t < t1) next_item(pre);
+  };
+  auto issue = [&](int stage) {
+    uint64_t mask = 0;
+    __syncwarp();                            // every lane has read the previous offsets
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if constexpr (kFp8) {
-          k[e] = static_cast<float>(static_cast<const __nv_fp8_e4m3*>(p.cache.k)[ko + e]);
-          v[e] = static_cast<float>(static_cast<const __nv_fp8_e4m3*>(p.cache.v)[vo + e]) * p.cache.v_scale;
+    for (int i = 0; i < kIds; ++i) {
+      const int r = lane + 32 * i;
+      longlong2 off = make_longlong2(-1, -1);
+      if (id_ok[i]) {
+        if (static_cast<unsigned>(id_page[i]) < static_cast<uint64_t>(p.cache.num_pages)) {
+          off.x = (id_page[i] * p.cache.k_page + id_at[i] * p.cache.k_slot + id_head * p.cache.k_head) * (kFp8 ? 1 : 2);
+          off.y = (id_page[i] * p.cache.v_page + id_at[i] * p.cache.v_slot + id_head * p.cache.v_head) * (kFp8 ? 1 : 2);
         } else {
-          k[e] = __bfloat162float(static_cast<const __nv_bfloat16*>(p.cache.k)[ko + e]);
-          v[e] = __bfloat162float(static_cast<const __nv_bfloat16*>(p.cache.v)[vo + e]);
+          record_error(kSiteBadIndex);
         }
       }
-      const float s = dot_warp(q, k);
-      const float mn = fmaxf(m, s);
-      const float a = expf(m - mn), x = expf(s - mn);
-      l = l * a + x;
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = acc[e] * a + x * v[e];
-      m = mn;
+      if (r < kTok) s_off[warp][r] = off;
+      mask |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, off.x >= 0)) << (32 * i);
     }
-    const float r = l > 0.0f ? 1.0f / l : 0.0f;
+    if (lane == 0) s_mask[warp][stage] = mask;
+    __syncwarp();
+    if (mask) {
+      const uint32_t dst = ring_a + stage * kDecStageBytes;
+      const int c = lane % Cfg::kChunks;
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      p.out[b * p.o_token + h * p.o_head + N * lane + e] = __float2bfloat16_rn(l > 0.0f ? acc[e] * r : 0.0f);
-    if (p.lse && lane == 0) p.lse[w] = l > 0.0f ? m + logf(l) : -INFINITY;
+      for (int i = 0; i < 8; ++i) {
+        const int r = lane / Cfg::kChunks + i * (32 / Cfg::kChunks);
+        const longlong2 off = s_off[warp][r];
+        const uint32_t n = off.x >= 0 ? 16u : 0u;
+        const int64_t ko = off.x >= 0 ? off.x + 16 * c : 0, vo = off.x >= 0 ? off.y + 16 * c : 0;
+        cp_async16(dst + dec_chunk<D, kFp8, false>(r, c), static_cast<const char*>(p.cache.k) + ko, n);
+        cp_async16(dst + kDecStageBytes / 2 + dec_chunk<D, kFp8, true>(r, c), static_cast<const char*>(p.cache.v) + vo, n);
+      }
+    }
+    cp_async_commit();
+  };
+
+  look_up();
+#pragma unroll
+  for (int s = 0; s < kDecStages - 1; ++s) {
+    issue(s);
+    look_up();
   }
+
+  int stage = 0;
+  int64_t t = t0;
+  while (t < t1) {
+    const int64_t seg = (cur.n - cur.j) < (t1 - t) ? (cur.n - cur.j) : (t1 - t);
+    const int hk = cur.sub / p.blocks, hb = cur.sub - hk * p.blocks;
+    const int h0 = hk * p.group + hb * 8 * kNT;            // first query head
+    const int heads = min(8 * kNT, p.group - hb * 8 * kNT);
+
+    // q as the B operand: lane (g, t4) holds head g's values.  bf16: as they
+    // lie.  e4m3 cache: f16, scaled by a power of two so that the largest is
+    // in [1, 2) (exact; what falls below 2^-24 of it is lost), k steps in the
+    // order of the k rows' 16-byte chunks.
+    uint32_t qf[kNT][kKT][2];
+    float sc[kNT][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int h = 8 * nt + g;
+      const __nv_bfloat16* src = p.q + cur.b * p.q_token + (h0 + h) * p.q_head;
+      const bool ok = h < heads;
+      if constexpr (!kFp8) {
+#pragma unroll
+        for (int k = 0; k < kKT; ++k) {
+          qf[nt][k][0] = ok ? __ldg(reinterpret_cast<const unsigned int*>(src + 16 * k + 2 * t4)) : 0u;
+          qf[nt][k][1] = ok ? __ldg(reinterpret_cast<const unsigned int*>(src + 16 * k + 8 + 2 * t4)) : 0u;
+        }
+        sc[nt][0] = sc[nt][1] = p.scale_log2;
+      } else {
+        float amax = 0.0f;
+        uint2 raw[kKT];
+#pragma unroll
+        for (int k = 0; k < kKT; ++k) {
+          raw[k] = ok ? __ldg(reinterpret_cast<const uint2*>(src + 16 * (t4 + 4 * (k / 4)) + 4 * (k % 4))) : make_uint2(0, 0);
+          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(raw[k].x)), fabsf(bf16_hi(raw[k].x))),
+                                   fmaxf(fabsf(bf16_lo(raw[k].y)), fabsf(bf16_hi(raw[k].y)))));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // 2^e <= amax < 2^(e+1); e from the exponent field, kept where 2^-e is normal too
+        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int k = 0; k < kKT; ++k) {
+          qf[nt][k][0] = pack2<true>(bf16_lo(raw[k].x) * down, bf16_hi(raw[k].x) * down);
+          qf[nt][k][1] = pack2<true>(bf16_lo(raw[k].y) * down, bf16_hi(raw[k].y) * down);
+        }
+        const float up = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        sc[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t4);
+        sc[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
+      }
+    }
+    float m[kNT][2], l[kNT][2], o[kNT][kMT][4];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+    }
+
+    for (int64_t step = 0; step < seg; ++step) {
+      cp_async_wait<kDecStages - 2>();
+      __syncwarp();
+      {
+        int ahead = stage + kDecStages - 1;
+        if (ahead >= kDecStages) ahead -= kDecStages;
+        issue(ahead);
+        look_up();
+      }
+      const uint32_t ka = ring_a + stage * kDecStageBytes, va = ka + kDecStageBytes / 2;
+      const uint64_t mask = s_mask[warp][stage];
+      if (++stage == kDecStages) stage = 0;
+      if (mask == 0) continue;
+      // ---- scores: s[nt][tt]: tokens 16 tt + g (+8), heads 2 t4 (+1) ----
+      float s[kNT][kTT][4];
+#pragma unroll
+      for (int tt = 0; tt < kTT; ++tt) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) s[nt][tt][0] = s[nt][tt][1] = s[nt][tt][2] = s[nt][tt][3] = 0.0f;
+        if constexpr (!kFp8) {
+#pragma unroll
+          for (int k = 0; k < kKT; ++k) {
+            uint32_t a[4];
+            ldsm4(a, ka + dec_chunk<D, kFp8, false>(16 * tt + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) mma16816<false>(s[nt][tt], a, qf[nt][k][0], qf[nt][k][1]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const uint4 r0 = lds128(ka + dec_chunk<D, kFp8, false>(16 * tt + g, t4 + 4 * c));
+            const uint4 r1 = lds128(ka + dec_chunk<D, kFp8, false>(16 * tt + g + 8, t4 + 4 * c));
+            const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t a[4] = {e4m3x2_to_f16x2(static_cast<uint16_t>(w0[k])), e4m3x2_to_f16x2(static_cast<uint16_t>(w1[k])),
+                                     e4m3x2_to_f16x2(static_cast<uint16_t>(w0[k] >> 16)),
+                                     e4m3x2_to_f16x2(static_cast<uint16_t>(w1[k] >> 16))};
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) mma16816<true>(s[nt][tt], a, qf[nt][4 * c + k][0], qf[nt][4 * c + k][1]);
+            }
+          }
+        }
+      }
+      // ---- softmax ----
+      const bool full = kTok == 64 ? mask == ~0ull : mask == (1ull << (kTok & 63)) - 1;
+      uint32_t pf[kNT][kTT][2];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < kTT; ++tt) {
+          s[nt][tt][0] *= sc[nt][0];
+          s[nt][tt][1] *= sc[nt][1];
+          s[nt][tt][2] *= sc[nt][0];
+          s[nt][tt][3] *= sc[nt][1];
+          if (!full) {
+            if (!((mask >> (16 * tt + g)) & 1)) s[nt][tt][0] = s[nt][tt][1] = -INFINITY;
+            if (!((mask >> (16 * tt + g + 8)) & 1)) s[nt][tt][2] = s[nt][tt][3] = -INFINITY;
+          }
+          mx0 = fmaxf(mx0, fmaxf(s[nt][tt][0], s[nt][tt][2]));
+          mx1 = fmaxf(mx1, fmaxf(s[nt][tt][1], s[nt][tt][3]));
+        }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+        }
+        mx0 = fmaxf(mx0, m[nt][0]);
+        mx1 = fmaxf(mx1, m[nt][1]);
+        if (__any_sync(0xffffffffu, mx0 > m[nt][0] || mx1 > m[nt][1])) {
+          const float a0 = m[nt][0] == -INFINITY ? 0.0f : ex2(m[nt][0] - mx0);
+          const float a1 = m[nt][1] == -INFINITY ? 0.0f : ex2(m[nt][1] - mx1);
+          m[nt][0] = mx0;
+          m[nt][1] = mx1;
+          l[nt][0] *= a0;
+          l[nt][1] *= a1;
+#pragma unroll
+          for (int i = 0; i < kMT; ++i) {
+            o[nt][i][0] *= a0;
+            o[nt][i][1] *= a1;
+            o[nt][i][2] *= a0;
+            o[nt][i][3] *= a1;
+          }
+        }
+        // the weights meet v in v's 16-bit type (bf16; f16 for an e4m3 cache):
+        // each is off by half an ulp at most, their sum l is of the unrounded
+        const float b0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+#pragma unroll
+        for (int tt = 0; tt < kTT; ++tt) {
+          const float p0 = ex2(s[nt][tt][0] - b0), p1 = ex2(s[nt][tt][1] - b1);
+          const float p2 = ex2(s[nt][tt][2] - b0), p3 = ex2(s[nt][tt][3] - b1);
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          pf[nt][tt][0] = movmatrix_t(pack2<kFp8>(p0, p1));
+          pf[nt][tt][1] = movmatrix_t(pack2<kFp8>(p2, p3));
+        }
+      }
+      // ---- o^T += v^T p^T ----
+#pragma unroll
+      for (int tt = 0; tt < kTT; ++tt) {
+        if constexpr (!kFp8) {
+#pragma unroll
+          for (int i = 0; i < kMT; ++i) {
+            uint32_t a[4];
+            ldsm4_t(a, va + dec_chunk<D, kFp8, true>(16 * tt + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) mma16816<false>(o[nt][i], a, pf[nt][tt][0], pf[nt][tt][1]);
+          }
+        } else {
+          // lane (g, t4) holds bytes g D/8 .. of tokens 2 t4, 2 t4 + 1, 2 t4 + 8,
+          // 2 t4 + 9; row g of the i-th product is value g D/8 + 2 i, row g + 8 the next
+          uint32_t w[4][D / 32];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = 16 * tt + 2 * t4 + (r & 1) + ((r >> 1) << 3);
+            if constexpr (D == 128) {
+              const uint4 x = lds128(va + dec_chunk<D, kFp8, true>(row, g));
+              w[r][0] = x.x;
+              w[r][1] = x.y;
+              w[r][2] = x.z;
+              w[r][3] = x.w;
+            } else {
+              const uint2 x = lds64(va + dec_chunk<D, kFp8, true>(row, g >> 1) + 8 * (g & 1));
+              w[r][0] = x.x;
+              w[r][1] = x.y;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kMT; ++i) {
+            const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;     // bytes 2i, 2i + 1 of both tokens, paired by byte
+            const uint32_t lo = __byte_perm(w[0][i >> 1], w[1][i >> 1], sel);
+            const uint32_t hi = __byte_perm(w[2][i >> 1], w[3][i >> 1], sel);
+            const uint32_t a[4] = {e4m3x2_to_f16x2(static_cast<uint16_t>(lo)), e4m3x2_to_f16x2(static_cast<uint16_t>(lo >> 16)),
+                                   e4m3x2_to_f16x2(static_cast<uint16_t>(hi)), e4m3x2_to_f16x2(static_cast<uint16_t>(hi >> 16))};
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) mma16816<true>(o[nt][i], a, pf[nt][tt][0], pf[nt][tt][1]);
+          }
+        }
+      }
+    }
+
+    // ---- the segment's result: the four warps joined, 4 heads at a time ----
+    const int64_t first = owner(item_t0), last = owner(item_t0 + cur.n - 1);
+    const bool whole = first == last;
+    float* slot = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == first ? 1 : 0)) * kSlot;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], x);
+        l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], x);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int h4 = 8 * nt + 4 * half;                  // heads h4 .. h4 + n4
+        const int n4 = min(4, heads - h4);
+        if (n4 <= 0) break;
+        if ((t4 >> 1) == half) {
+          const int h = 2 * (t4 & 1);
+          float* so = s_o + (warp * 4 + h) * Cfg::kPad;
+#pragma unroll
+          for (int i = 0; i < kMT; ++i) {
+            const int d0 = kFp8 ? g * (D / 8) + 2 * i : 16 * i + g;
+            const int d1 = kFp8 ? d0 + 1 : d0 + 8;
+            so[d0] = o[nt][i][0];
+            so[d1] = o[nt][i][2];
+            so[Cfg::kPad + d0] = o[nt][i][1];
+            so[Cfg::kPad + d1] = o[nt][i][3];
+          }
+          if (g == 0) {
+            s_m[warp][h] = m[nt][0];
+            s_m[warp][h + 1] = m[nt][1];
+            s_l[warp][h] = l[nt][0];
+            s_l[warp][h + 1] = l[nt][1];
+          }
+        }
+        __syncthreads();
+        for (int i = tid; i < n4 * (D / 4); i += kDecThreads) {
+          const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+          float mm = s_m[0][h];
+#pragma unroll
+          for (int w = 1; w < kDecWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
+          float ll = 0.0f;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int w = 0; w < kDecWarps; ++w) {
+            const float a = s_m[w][h] == -INFINITY ? 0.0f : ex2(s_m[w][h] - mm);
+            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 4 + h) * Cfg::kPad + d);
+            ll += a * s_l[w][h];
+            v.x += a * x.x;
+            v.y += a * x.y;
+            v.z += a * x.z;
+            v.w += a * x.w;
+          }
+          if (whole) {
+            dec_store<D>(p, cur.b, h0 + h4 + h, d, v, mm, ll);
+          } else {
+            *reinterpret_cast<float4*>(slot + (h4 + h) * D + d) = v;
+            if (d == 0) {
+              slot[8 * kNT * D + h4 + h] = mm;
+              slot[8 * kNT * (D + 1) + h4 + h] = ll;
+            }
+          }
+        }
+        __syncthreads();
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomic_add_acq_rel_gpu(p.counters + first, 1) == last - first;
+      __syncthreads();
+      if (s_last) {
+        // join the ranges' partial results in range order: warp w takes
+        // ranges w, w + 4, ...; then the warps in order
+        __threadfence();
+        if (tid == 0) p.counters[first] = 0;
+        const int n = static_cast<int>(last - first) + 1;
+        auto part = [&](int i) {
+          return p.partials + (static_cast<int64_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * kSlot;
+        };
+        constexpr int kLanes = D / 4;            // lanes per head
+        constexpr int kPer = 32 / kLanes;        // heads at once
+        for (int hh0 = 0; hh0 < heads; hh0 += kPer) {
+          const int hh = hh0 + lane / kLanes, d = (lane % kLanes) * 4;
+          const bool ok = hh < heads;
+          float mm = -INFINITY;
+          for (int i = lane % kLanes; ok && i < n; i += kLanes) mm = fmaxf(mm, __ldcg(part(i) + 8 * kNT * D + hh));
+#pragma unroll
+          for (int x = kLanes / 2; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+          float ll = 0.0f;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (ok) {
+#pragma unroll 4
+            for (int i = warp; i < n; i += kDecWarps) {
+              const float* q = part(i);
+              const float mi = __ldcg(q + 8 * kNT * D + hh), li = __ldcg(q + 8 * kNT * (D + 1) + hh);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(q + hh * D + d));
+              const float a = mi == -INFINITY ? 0.0f : ex2(mi - mm);
+              ll += a * li;
+              v.x += a * x.x;
+              v.y += a * x.y;
+              v.z += a * x.z;
+              v.w += a * x.w;
+            }
+            *reinterpret_cast<float4*>(s_o + (warp * kPer + lane / kLanes) * D + d) = v;
+            if (d == 0) s_l[warp][lane / kLanes] = ll;
+          }
+          __syncthreads();
+          if (warp == 0 && ok) {
+            ll = 0.0f;
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kDecWarps; ++w) {
+              const float4 x = *reinterpret_cast<const float4*>(s_o + (w * kPer + lane / kLanes) * D + d);
+              ll += s_l[w][lane / kLanes];
+              v.x += x.x;
+              v.y += x.y;
+              v.z += x.z;
+              v.w += x.w;
+            }
+            dec_store<D>(p, cur.b, h0 + hh, d, v, mm, ll);
+          }
+          __syncthreads();
+        }
+      }
+    }
+    t += seg;
+    item_t0 += cur.n;
+    if (t < t1) next_item(cur);
+  }
+  cp_async_wait<0>();
   grid_launch_dependents();
 }
 

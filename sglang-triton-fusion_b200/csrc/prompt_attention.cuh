@@ -23,6 +23,16 @@ struct PromptParams {
   int causal;
 };
 
+template <int N>
+__device__ __forceinline__ float dot_warp(const float (&a)[N], const float (&b)[N]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) s += a[e] * b[e];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
 __device__ __forceinline__ int cut(int x, int hi) {
   if (x < 0 || x > hi) {
     record_error(kSiteBadIndex);

@@ -77,6 +77,30 @@ int check_rows(const void* p, int64_t token, int64_t head, int tokens, int heads
   return FP8GQ_OK;
 }
 
+// ----------------------------------------------------------------- decode --
+constexpr int kDecCtasPerSm = 2;
+static_assert(kDecCounterBytes / 4 >= 1024, "a counter per CTA");
+
+size_t decode_workspace_bytes(int group, int D, int sm_count) {
+  return kDecCounterBytes +
+         static_cast<size_t>(kDecCtasPerSm) * sm_count * 2 * dec_slot_floats(D, group > 8 ? 2 : 1) * sizeof(float);
+}
+
+template <int D, bool kFp8, int kNT>
+cudaError_t launch_decode(const DecodeParams& p, const DeviceInfo& di, fp8gq_stream_t stream) {
+  using Cfg = DecCfg<D, kFp8>;
+  auto fn = paged_decode_kernel<D, kFp8, kNT>;
+  cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(fn), static_cast<int>(Cfg::kSmem));
+  if (e != cudaSuccess) return e;
+  // no more CTAs than tiles, were every sequence as long as its page table
+  const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.cache.page_size + Cfg::kTile - 1) / Cfg::kTile;
+  int64_t grid = kDecCtasPerSm * di.sm_count;
+  const int64_t most = tiles > grid ? grid : tiles * p.Hkv * p.blocks * p.B;
+  if (most < grid) grid = most < 1 ? 1 : most;
+  return launch_with_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(kDecThreads), Cfg::kSmem,
+                         static_cast<cudaStream_t>(stream), p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -132,10 +156,9 @@ int fp8gq_qk_norm_rope_append(const void* qkv, int64_t ldqkv, const int64_t* pos
 }
 
 size_t fp8gq_paged_decode_workspace_bytes(int Hq, int Hkv, int D) {
-  (void)Hq;
-  (void)Hkv;
-  (void)D;
-  return 0;
+  DeviceInfo di;
+  if (check_heads(Hq, Hkv, D) != FP8GQ_OK || device_info(&di, nullptr) != FP8GQ_OK) return 0;
+  return decode_workspace_bytes(Hq / Hkv, D, di.sm_count);
 }
 
 int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -173,14 +196,26 @@ int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t 
   p.B = B;
   p.Hq = Hq;
   p.Hkv = Hkv;
-  p.scale = scale;
-  const int64_t blocks = (static_cast<int64_t>(B) * Hq + 3) / 4;
-  if (blocks > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
   const bool fp8 = cache->dtype == FP8GQ_DTYPE_E4M3;
-  auto fn = D == 128 ? (fp8 ? paged_decode_kernel<128, true> : paged_decode_kernel<128, false>)
-                     : (fp8 ? paged_decode_kernel<64, true> : paged_decode_kernel<64, false>);
-  const cudaError_t e = launch_with_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(128), 0,
-                                        static_cast<cudaStream_t>(stream), p);
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (cache->page_size == 1 << i) p.page_shift = i;
+  p.group = Hq / Hkv;
+  const int nt = p.group > 8 ? 2 : 1;
+  p.blocks = (p.group + 8 * nt - 1) / (8 * nt);
+  p.scale_log2 = scale * 1.4426950408889634f * (fp8 ? cache->k_scale : 1.0f);
+  p.out_scale = fp8 ? cache->v_scale : 1.0f;
+  if (!workspace || workspace_bytes < decode_workspace_bytes(p.group, D, di.sm_count)) return FP8GQ_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return FP8GQ_ERR_ALIGNMENT;
+  p.counters = static_cast<int*>(workspace);
+  p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kDecCounterBytes);
+  cudaError_t e;
+  if (D == 128)
+    e = fp8 ? (nt == 2 ? launch_decode<128, true, 2>(p, di, stream) : launch_decode<128, true, 1>(p, di, stream))
+            : (nt == 2 ? launch_decode<128, false, 2>(p, di, stream) : launch_decode<128, false, 1>(p, di, stream));
+  else
+    e = fp8 ? (nt == 2 ? launch_decode<64, true, 2>(p, di, stream) : launch_decode<64, true, 1>(p, di, stream))
+            : (nt == 2 ? launch_decode<64, false, 2>(p, di, stream) : launch_decode<64, false, 1>(p, di, stream));
   return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_paged_decode_attention");
 }
 

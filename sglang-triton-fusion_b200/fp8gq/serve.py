@@ -26,6 +26,7 @@ HEAD_DIMS = (64, 128)
 MAX_TOP = 32
 _BF16, _E4M3, _F32 = 0, 1, 2   # FP8GQ_DTYPE_*
 _byref = ctypes.byref
+_decode_ws_bytes: dict = {}    # (device, Hq, Hkv, D) -> fp8gq_paged_decode_workspace_bytes
 
 
 def _check_cache(k, v, k_scale, v_scale):
@@ -141,8 +142,11 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     lib = _lib.load()
     stream = _stream(dev)
-    nbytes = lib.fp8gq_paged_decode_workspace_bytes(hq, hkv, d)
-    ws_ptr, ws_n = _workspace_entry(dev, nbytes, stream)[1:] if nbytes else (None, 0)
+    key = (dev.index, hq, hkv, d)
+    nbytes = _decode_ws_bytes.get(key)
+    if nbytes is None:
+        nbytes = _decode_ws_bytes[key] = lib.fp8gq_paged_decode_workspace_bytes(hq, hkv, d)
+    _, ws_ptr, ws_n = _workspace_entry(dev, nbytes, stream)
     st = lib.fp8gq_paged_decode_attention(
         q.data_ptr(), qs[0], qs[1], _byref(cache), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
         lens.data_ptr(), out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(), b, hq, hkv, d,
