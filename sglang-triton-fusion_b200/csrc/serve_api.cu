@@ -2,6 +2,8 @@
 // checks, kernel selection and launch.
 #include <cuda_runtime.h>
 
+#include <cmath>
+
 #include "../../include/fp8gq.h"
 #include "fp8gq_device.cuh"
 #include "host_common.h"
@@ -75,6 +77,25 @@ int check_rows(const void* p, int64_t token, int64_t head, int tokens, int heads
   if ((tokens > 1 && token < D) || (heads > 1 && head < D)) return FP8GQ_ERR_STRIDE;
   if (!aligned16(p) || token % 8 || head % 8) return FP8GQ_ERR_ALIGNMENT;
   return FP8GQ_OK;
+}
+
+// ----------------------------------------------------------------- prompt --
+// [tokens, heads, D] bf16 as boxes of 64 values x `box_heads` heads x
+// `box_tokens` tokens, 128-byte swizzle.  A stride that no coordinate above 0
+// uses is replaced by a valid one.
+bool make_heads_tmap(CUtensorMap* map, const void* p, int tokens, int heads, int D, int64_t token, int64_t head,
+                     int box_heads, int box_tokens) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  if (heads == 1) head = D;
+  if (tokens == 1) token = static_cast<int64_t>(heads) * head;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head) * 2, static_cast<cuuint64_t>(token) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // ----------------------------------------------------------------- decode --
@@ -237,18 +258,12 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
   DeviceInfo di;
   st = device_info(&di, nullptr);
   if (st != FP8GQ_OK) return st;
+  if (!std::isfinite(scale)) return FP8GQ_ERR_UNSUPPORTED;
+  const int group = Hq / Hkv;
+  if (group > 128) return FP8GQ_ERR_UNSUPPORTED;
   PromptParams p{};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
-  p.v = static_cast<const __nv_bfloat16*>(v);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
-  p.q_token = q_token_stride;
-  p.q_head = q_head_stride;
-  p.k_token = k_token_stride;
-  p.k_head = k_head_stride;
-  p.v_token = v_token_stride;
-  p.v_head = v_head_stride;
   p.o_token = o_token_stride;
   p.o_head = o_head_stride;
   p.cu_q = cu_q;
@@ -258,13 +273,26 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
   p.Tk = Tk;
   p.Hq = Hq;
   p.Hkv = Hkv;
-  p.scale = scale;
+  p.group = group;
+  p.rows = 128 / group;
+  // a scale of 0 as one too small to tell scores apart, so that -inf stays -inf
+  p.scale_log2 = scale == 0.0f ? 1e-30f : std::fabs(scale) * 1.4426950408889634f;
+  p.negate = scale < 0.0f;
   p.causal = causal ? 1 : 0;
-  const int64_t blocks = (static_cast<int64_t>(Tq) * Hq + 3) / 4;
+  CUtensorMap tq, tk, tv;
+  if (!make_heads_tmap(&tq, q, Tq, Hq, D, q_token_stride, q_head_stride, group, p.rows) ||
+      !make_heads_tmap(&tk, Tk ? k : q, Tk ? Tk : 1, Hkv, D, Tk ? k_token_stride : 0, Tk ? k_head_stride : D, 1, kPrKeys) ||
+      !make_heads_tmap(&tv, Tk ? v : q, Tk ? Tk : 1, Hkv, D, Tk ? v_token_stride : 0, Tk ? v_head_stride : D, 1, kPrKeys))
+    return FP8GQ_ERR_LAUNCH;
+  // a row block more than the tokens fill for each sequence's odd end
+  const int64_t blocks = (static_cast<int64_t>(Tq) / (2 * p.rows) + B) * Hkv;
   if (blocks > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
   auto fn = D == 128 ? prompt_attention_kernel<128> : prompt_attention_kernel<64>;
-  const cudaError_t e = launch_with_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(128), 0,
-                                        static_cast<cudaStream_t>(stream), p);
+  const size_t smem = D == 128 ? PrCfg<128>::kSmem : PrCfg<64>::kSmem;
+  cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(fn), static_cast<int>(smem));
+  if (e == cudaSuccess)
+    e = launch_with_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(kPrThreads), smem,
+                        static_cast<cudaStream_t>(stream), tq, tk, tv, p);
   return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_prompt_attention");
 }
 
