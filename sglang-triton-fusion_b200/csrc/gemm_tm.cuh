@@ -1328,22 +1328,6 @@ inline bool cached_tmap(CUtensorMap* map, int kind, const void* ptr, int rows, i
   return true;
 }
 
-// cudaFuncAttributeNonPortableClusterSizeAllowed set once per kernel and
-// device, before a cluster of more than 8 CTAs is queried or launched.
-inline cudaError_t ensure_nonportable_clusters(const void* fn) {
-  static std::mutex mu;
-  static std::map<std::pair<int, const void*>, bool> done;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const auto key = std::make_pair(dev, fn);
-  std::lock_guard<std::mutex> lock(mu);
-  if (done.count(key)) return cudaSuccess;
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) done[key] = true;
-  return e;
-}
-
 // Shared-memory plan of one pass: ring depth, activation mode and layout.
 struct TmPlan {
   int stages, npw, resident;

@@ -96,6 +96,22 @@ inline cudaError_t ensure_max_smem(const void* fn, int max_smem) {
   return cudaSuccess;
 }
 
+// cudaFuncAttributeNonPortableClusterSizeAllowed set once per kernel and
+// device, before a cluster of more than 8 CTAs is queried or launched.
+inline cudaError_t ensure_nonportable_clusters(const void* fn) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, bool> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const auto key = std::make_pair(dev, fn);
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count(key)) return cudaSuccess;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done[key] = true;
+  return e;
+}
+
 // The error word and the wait limit are device variables, of which each
 // translation unit with bounded waits has its own; these read, clear and set
 // the serving operators' (serve_api.cu), for fp8gq_device_error and

@@ -98,6 +98,15 @@ bool make_heads_tmap(CUtensorMap* map, const void* p, int tokens, int heads, int
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// ---------------------------------------------------------- log probabilities --
+// CTAs per row: enough to fill the GPU (4 per SM), each with 4096 values at
+// least, 16 at most.
+int logprobs_cluster(int T, int V, int sm_count) {
+  int c = 1;
+  while (c < 16 && static_cast<int64_t>(T) * c < 4 * sm_count && V / (2 * c) >= 4096) c *= 2;
+  return c;
+}
+
 // ----------------------------------------------------------------- decode --
 constexpr int kDecCtasPerSm = 2;
 static_assert(kDecCounterBytes / 4 >= 1024, "a counter per CTA");
@@ -302,6 +311,7 @@ int fp8gq_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_
   if (T < 0 || V < 1 || top_k < 0 || top_k > V) return FP8GQ_ERR_SHAPE;
   if (top_k > kMaxTop || (dtype != FP8GQ_DTYPE_BF16 && dtype != FP8GQ_DTYPE_F32)) return FP8GQ_ERR_UNSUPPORTED;
   if (T == 0) return FP8GQ_OK;
+  if (T > INT32_MAX / 16) return FP8GQ_ERR_UNSUPPORTED;
   if (!logits || (logprobs && !tokens) || (top_k > 0 && (!top_ids || !top_logprobs))) return FP8GQ_ERR_NULL_POINTER;
   if (T > 1 && ld < V) return FP8GQ_ERR_STRIDE;
   if (reinterpret_cast<uintptr_t>(logits) & (dtype == FP8GQ_DTYPE_BF16 ? 1u : 3u)) return FP8GQ_ERR_ALIGNMENT;
@@ -320,7 +330,11 @@ int fp8gq_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_
   p.V = V;
   p.K = top_k;
   auto fn = dtype == FP8GQ_DTYPE_BF16 ? token_logprobs_kernel<__nv_bfloat16> : token_logprobs_kernel<float>;
-  const cudaError_t e = launch_with_pdl(fn, dim3(T), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
+  p.cluster = logprobs_cluster(T, V, di.sm_count);
+  cudaError_t e = p.cluster > 8 ? ensure_nonportable_clusters(reinterpret_cast<const void*>(fn)) : cudaSuccess;
+  if (e == cudaSuccess)
+    e = launch_with_pdl_cluster(fn, dim3(static_cast<unsigned>(T) * p.cluster), dim3(kLpThreads), 0,
+                                static_cast<cudaStream_t>(stream), p.cluster, p);
   return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_token_logprobs");
 }
 
