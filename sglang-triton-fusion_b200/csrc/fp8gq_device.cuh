@@ -37,6 +37,7 @@ enum ErrorSite : unsigned int {
   kSiteStackRing = 9,    // stack runner: a ring, accumulator or scale wait inside a CTA
   kSiteStackDep = 10,    // stack runner: waiting for every CTA to finish an earlier linear
   kSitePrompt = 11,      // prompt attention: a ring, score or accumulator wait inside a CTA
+  kSiteScore = 13,       // token log probabilities: waiting for a step of the stream
   kSiteBadIndex = 12,    // a serving operator met a position, slot, page, length, offset or token out of range
 };
 

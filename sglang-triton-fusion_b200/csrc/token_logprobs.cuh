@@ -7,7 +7,7 @@
 // Each thread keeps (r, s, e) of what it has read, rescaled when r moves; such
 // triples join in any grouping.
 //
-// Bound: HBM, one pass; next to it the exponentials (one MUFU operation per
+// Bound: HBM, one pass, streamed through a ring of bulk copies; next to it the exponentials (one MUFU operation per
 // value, 16 a cycle and SM: 72 % of the time that a bf16 row takes to arrive),
 // so the rest is kept to packed pairs: clamp, fma, add, fma.
 //
@@ -34,6 +34,8 @@ constexpr int kLpThreads = 32 * kLpWarps;
 constexpr int kLpUnroll = 4;              // 16-byte vectors per lane and chunk (32 bf16 or 16 fp32 values)
 constexpr int kLpParts = 4;               // columns per thread: what it reads in this many parts
 constexpr int kLpPool = 512;              // candidates of a CTA
+constexpr int kLpStages = 3;              // steps of the CTA (16 KB) in flight
+constexpr int kLpStepBytes = kLpThreads * kLpUnroll * 16;
 
 struct LogprobParams {
   const void* logits;
@@ -169,11 +171,15 @@ __device__ __forceinline__ LpSums lp_join_lanes(LpSums a, int n, int lane) {
 template <typename T>
 struct LpChunk {
   uint32_t w[4 * kLpUnroll];
-  __device__ __forceinline__ void load(const uint4* vec, int v, int v_hi) {
+  // from shared memory; `left` vectors of the CTA's step are there
+  __device__ __forceinline__ void load(uint32_t step, int v, int left) {
     constexpr uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
-      const uint4 a = v + 32 * u < v_hi ? __ldcg(vec + v + 32 * u) : make_uint4(none, none, none, none);
+      uint4 a = make_uint4(none, none, none, none);
+      if (v + 32 * u < left)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w)
+                     : "r"(step + 16 * (v + 32 * u)) : "memory");
       w[4 * u] = a.x;
       w[4 * u + 1] = a.y;
       w[4 * u + 2] = a.z;
@@ -383,12 +389,18 @@ template <typename T>
 __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobParams p) {
   constexpr int kVec = 16 / sizeof(T);
   constexpr int kStep = kLpThreads * kLpUnroll;
+  extern __shared__ __align__(128) unsigned char ring[];      // the stream's steps; the candidates once it has ended
+  struct Found {
+    lp_key pool[kLpPool];
+    lp_key list[kLpWarps][32];
+    float max[kLpWarps][32];
+    uint16_t column[kLpParts * kLpThreads];
+  };
+  static_assert(sizeof(Found) <= kLpStages * kLpStepBytes, "the candidates fit the ring");
+  Found& found = *reinterpret_cast<Found*>(ring);
+  __shared__ uint64_t s_full[kLpStages], s_free[kLpStages];
   __shared__ lp_key s_out[32];                   // this CTA's best, read by the cluster
-  __shared__ lp_key s_pool[kLpPool];
-  __shared__ lp_key s_list[kLpWarps][32];
-  __shared__ float s_max[kLpWarps][32];
   __shared__ float s_part[kLpParts][kLpThreads];
-  __shared__ uint16_t s_column[kLpParts * kLpThreads];
   __shared__ LpSums s_sum[kLpWarps], s_total;
   __shared__ int s_columns, s_found, s_regular;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -397,6 +409,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   const int K = p.K;
   if (tid == 0) s_columns = s_found = 0;         // used after the barriers of lp_kth
   if (tid < 32) s_out[tid] = 0;
+  if (tid == 0) {
+    for (int i = 0; i < kLpStages; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], kLpWarps);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
   grid_dependency_wait();
 
   // a row: up to kVec - 1 values before the first 16-byte boundary, vectors, up to kVec - 1 after
@@ -411,12 +431,18 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   // the stream
   LpSums sum = {kLpFloor, 0.0f, 0.0f};
   float2 s2 = make_float2(0.0f, 0.0f), e2 = make_float2(0.0f, 0.0f);
-  const int v_warp = v_lo + warp * 32 * kLpUnroll;
   const int its = (v_hi - v_lo + kStep - 1) / kStep, part_its = (its + kLpParts - 1) / kLpParts;
   float most = -INFINITY, part = -INFINITY;
   int it = 0, parts = 0;
-  LpChunk<T> now;
-  now.load(vec, v_warp + lane, v_hi);
+  const uint64_t policy = l2_policy_evict_first();
+  auto copy = [&](int i, int stage) {            // step i of this CTA
+    const int n = min(kStep, v_hi - v_lo - i * kStep);
+    mbar_arrive_expect_tx(&s_full[stage], 16 * n);
+    bulk_g2s(ring + stage * kLpStepBytes, vec + v_lo + i * kStep, 16 * n, &s_full[stage], policy);
+  };
+  bool ok = true;
+  if (tid == 0)
+    for (int i = 0; i < min(kLpStages, its); ++i) copy(i, i);
   // the given token's logit, fetched meanwhile
   int64_t token = -1;
   float token_logit = 0.0f;
@@ -425,9 +451,23 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     if (token >= p.V) record_error(kSiteBadIndex);
     else if (token >= 0) token_logit = logit_at(row, token);
   }
-  for (int v0 = v_warp; v0 < v_hi; v0 += kStep) {
-    LpChunk<T> next;
-    if (v0 + kStep < v_hi) next.load(vec, v0 + kStep + lane, v_hi);
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int i = 0; i < its; ++i) {
+    LpChunk<T> now;
+    ok = mbar_wait_warp(&s_full[stage], phase, kSiteScore, lane) && ok;
+    now.load(smem_u32(ring) + stage * kLpStepBytes, warp * 32 * kLpUnroll + lane, ok ? v_hi - v_lo - i * kStep : 0);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s_free[stage]);
+    // the stage of the step before, which every warp has read by now or soon
+    if (tid == 0 && i > 0 && i - 1 + kLpStages < its) {
+      const int before_stage = stage == 0 ? kLpStages - 1 : stage - 1;
+      if (mbar_wait(&s_free[before_stage], stage == 0 ? phase ^ 1 : phase, kSiteScore)) copy(i - 1 + kLpStages, before_stage);
+    }
+    if (++stage == kLpStages) {
+      stage = 0;
+      phase ^= 1;
+    }
     const float mx = now.max();
     part = fmaxf(part, mx);
     if (++it == part_its) {
@@ -445,7 +485,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       sum.m = r;
     }
     now.add(sum.m, s2, e2);
-    now = next;
   }
   if (it > 0) {
     s_part[parts++][tid] = part;
@@ -457,7 +496,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   // the candidates
   float low = -INFINITY;
   if (K > 0) {
-    low = just_below(float_order(lp_kth(most, K, s_max, warp, lane)));
+    __syncthreads();                             // the ring has been read
+    low = just_below(float_order(lp_kth(most, K, found.max, warp, lane)));
     // the columns to read again, listed (in any order)
     unsigned is[kLpParts];
     int here = 0;
@@ -473,7 +513,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
 #pragma unroll
       for (int i = 0; i < kLpParts; ++i) {
         if ((is[i] >> lane) & 1)
-          s_column[at + __popc(is[i] & ((1u << lane) - 1))] = static_cast<uint16_t>(i * kLpThreads + tid);
+          found.column[at + __popc(is[i] & ((1u << lane) - 1))] = static_cast<uint16_t>(i * kLpThreads + tid);
         at += __popc(is[i]);
       }
     }
@@ -482,14 +522,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     const int deep = kLpUnroll * part_its;       // vectors of a column, at most
     const int again = s_columns * deep;
     for (int f = tid; f < again; f += kLpThreads) {
-      const int col = f / deep, c = s_column[col] % kLpThreads;
-      const int j = f - col * deep + deep * (s_column[col] / kLpThreads);
+      const int col = f / deep, c = found.column[col] % kLpThreads;
+      const int j = f - col * deep + deep * (found.column[col] / kLpThreads);
       const int v = v_lo + (c & ~31) * kLpUnroll + (c & 31) + 32 * (j % kLpUnroll) + kStep * (j / kLpUnroll);
       if (v < v_hi) {
         const uint4 a = __ldcg(vec + v);
         const T* x = reinterpret_cast<const T*>(&a);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) lp_keep(logit_at(x, i), before + v * kVec + i, low, &s_found, s_pool);
+        for (int i = 0; i < kVec; ++i) lp_keep(logit_at(x, i), before + v * kVec + i, low, &s_found, found.pool);
       }
     }
   }
@@ -502,7 +542,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     const float y = __fmaf_rn(c, kLog2e, -sum.m), f = lp_ex2(y);
     sum.s += f;
     sum.e = __fmaf_rn(f, y, sum.e);
-    if (K > 0) lp_keep(x, id, low, &s_found, s_pool);
+    if (K > 0) lp_keep(x, id, low, &s_found, found.pool);
   }
 
   // the warps, in order
@@ -514,15 +554,15 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     if (n <= kLpPool) {
       // a candidate's place: how many are above it
       for (int i = tid; i < n; i += kLpThreads) {
-        const lp_key x = s_pool[i];
+        const lp_key x = found.pool[i];
         int above = 0;
-        for (int j = 0; j < n; ++j) above += s_pool[j] > x;
+        for (int j = 0; j < n; ++j) above += found.pool[j] > x;
         if (above < K) s_out[above] = x;
       }
     } else {
       __syncthreads();
       lp_by_passes(row, before + v_lo * kVec, before + v_hi * kVec, rank == 0 ? before : 0, rank == 0 ? after : p.V, p.V,
-                   K, s_out, s_pool);
+                   K, s_out, found.pool);
     }
   }
   if (warp == 0) {
@@ -546,8 +586,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
           asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(b) : "r"(at) : "memory");
           a = lp_merge(a, b, lane);
         }
-        s_list[warp][lane] = a;
-        key = lp_merge_lists(s_list, warp, lane);
+        found.list[warp][lane] = a;
+        key = lp_merge_lists(found.list, warp, lane);
       }
       if (warp == 0) {
         LpSums o = {kLpFloor, 0.0f, 0.0f};
@@ -602,7 +642,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     }
   }
   __syncthreads();
-  if (!s_regular) lp_irregular(p, row, t, s_pool, s_sum);
+  if (!s_regular) lp_irregular(p, row, t, found.pool, s_sum);
   grid_launch_dependents();
 }
 
