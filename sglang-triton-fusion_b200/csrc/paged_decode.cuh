@@ -9,17 +9,21 @@
 //
 // Work split: the tiles (4 warps x kTok tokens of one sequence and kv head) of
 // all sequences form one flat list, cut into equal contiguous ranges, one per
-// CTA, two CTAs per SM.  The lengths are read on the device (a captured step
+// CTA, two CTAs per SM; the start of each (sequence, head) counts as
+// kDecItemCost tiles more.  The lengths are read on the device (a captured step
 // replays while they grow), so ragged batches and long single sequences
 // balance the same way.  A (sequence, head) that lies in several ranges leaves
 // partial results in the workspace; the last CTA to arrive joins them in range
 // order, so the result does not depend on who is last.
 //
-// Inside a CTA each warp runs alone: it copies its own kTok rows of k and v
-// (8 KB per stage, 16-byte cp.async, kStages stages) and computes on them with
-// matrix instructions whose M side is the tokens (S^T = K Q^T, 16 x 8) and
-// then the head's values (O^T = V^T P^T), so a group of up to 8 query heads
-// wastes nothing of K and V and no barrier stands in the loop.
+// Inside a CTA each warp runs alone: its lanes look up the pages of its own
+// kTok tokens and copy their rows of k and v (8 KB per step, kDecStages steps in
+// flight), and it computes on them with matrix instructions whose M side is the
+// tokens (S^T = K Q^T, 16 x 8) and then the head's values (O^T = V^T P^T), so a
+// group of up to 8 query heads wastes nothing of K and V and no barrier stands
+// in the loop.  The copies are 16-byte cp.async: any page size and stride, and
+// one bulk copy per row was measured at 16 cycles each (8 x 32768 tokens, e4m3:
+// 235 us against 131).
 #pragma once
 
 #include "fp8gq_device.cuh"
@@ -52,36 +56,35 @@ struct DecodeParams {
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecStages = 3;
-constexpr int kDecStageBytes = 8192;        // k and v rows of one warp's step
+constexpr int kDecStepBytes = 8192;         // k and v rows of one warp's step
 constexpr int kDecCounterBytes = 16384;     // the workspace's counters (the tile kernel's too)
 constexpr int kDecMinTiles = 2;             // tiles per CTA below which fewer CTAs work
+constexpr int kDecItemCost = 1;             // what starting a (sequence, head) counts, in tiles
 
 template <int D, bool kFp8>
 struct DecCfg {
   static constexpr int kRow = D * (kFp8 ? 1 : 2);       // bytes of a row
-  static constexpr int kTok = kDecStageBytes / 2 / kRow;
+  static constexpr int kTok = kDecStepBytes / 2 / kRow;
   static constexpr int kTile = kTok * kDecWarps;
   static constexpr int kChunks = kRow / 16;
+  // distance of rows in shared memory: rows read by one phase of a load fall on
+  // different banks (the e4m3 k rows: pairs of rows meet, two phases more)
+  static constexpr int kRowK = kFp8 ? kRow : kRow + 16;
+  static constexpr int kRowV = kRow + 16;
+  static constexpr int kStage = kTok * (kRowK + kRowV);
   static constexpr int kPad = D + 4;                    // o in shared memory: conflict-free fragment writes
-  static constexpr size_t kSmem = static_cast<size_t>(kDecWarps) * kDecStages * kDecStageBytes +
-                                  sizeof(float) * kDecWarps * 4 * kPad;
+  static constexpr size_t kSmem = static_cast<size_t>(kDecWarps) * kDecStages * kStage +
+                                  sizeof(float) * kDecWarps * 2 * kPad;
 };
 
 // Floats of one partial result: o [8 NT][D], m [8 NT], l [8 NT].
 inline __host__ __device__ constexpr int dec_slot_floats(int D, int NT) { return 8 * NT * (D + 2); }
 
-// Where 16-byte chunk c of row r lies: rows read by one phase of a shared-memory
-// load fall on different banks.
-template <int D, bool kFp8, bool kIsV>
-__device__ __forceinline__ uint32_t dec_chunk(int r, int c) {
-  constexpr int kRow = DecCfg<D, kFp8>::kRow;
-  if constexpr (!kFp8) return r * kRow + ((c ^ (r & 7)) << 4);
-  else if constexpr (D == 128) return r * kRow + ((kIsV ? c ^ (r & 6) : c ^ ((r & 1) << 2)) << 4);
-  else return r * kRow + ((kIsV ? c ^ ((r >> 1) & 3) : c) << 4);
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -167,10 +170,13 @@ __device__ __forceinline__ void dec_store(const DecodeParams& p, int b, int h, i
     p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// A place in the flat list of tiles.
-struct DecCursor {
-  int b, sub, j;       // sequence, (kv head, head block), tile of the sequence
+// Where a CTA is in the flat list: (sequence b, kv head and head block sub) and
+// its tiles [j, j_end) that are this CTA's.
+struct DecWalk {
+  int b, sub, j, j_end;
   int len, n;          // the sequence's tokens and tiles
+  int64_t start;       // of the item in the flat list
+  bool done;
 };
 
 template <int D, bool kFp8, int kNT>
@@ -178,27 +184,31 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
   using Cfg = DecCfg<D, kFp8>;
   constexpr int kTok = Cfg::kTok, kTile = Cfg::kTile, kMT = D / 16, kKT = D / 16, kTT = kTok / 16;
   constexpr int kSlot = dec_slot_floats(D, kNT);
+  constexpr int kRowK = Cfg::kRowK, kRowV = Cfg::kRowV;
+  constexpr uint64_t kFull = kTok == 64 ? ~0ull : (1ull << (kTok & 63)) - 1;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t s_scan[kDecThreads];
   __shared__ int64_t s_wsum[kDecWarps];
-  __shared__ uint64_t s_mask[kDecWarps][kDecStages];
-  __shared__ longlong2 s_off[kDecWarps][kTok];
-  __shared__ float s_m[kDecWarps][4], s_l[kDecWarps][4];
+  __shared__ uint2 s_off[kDecWarps][kTok];                // a step's rows of k and v, in 16 bytes from the cache's base
+  __shared__ uint64_t s_mask[kDecWarps][kDecStages];      // a step's tokens that count
+  __shared__ float s_m[kDecWarps][2], s_l[kDecWarps][2];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  unsigned char* ring = smem + warp * (kDecStages * kDecStageBytes);
-  const uint32_t ring_a = smem_u32(ring);
-  float* s_o = reinterpret_cast<float*>(smem + kDecWarps * kDecStages * kDecStageBytes);
+  const uint32_t ring = smem_u32(smem) + warp * (kDecStages * Cfg::kStage);
+  float* s_o = reinterpret_cast<float*>(smem + kDecWarps * kDecStages * Cfg::kStage);
   const int items = p.Hkv * p.blocks;
 
   grid_dependency_wait();
 
-  // ---- the flat list: tiles of the sequences before each thread's share ----
+  // ---- the flat list: what lies before each thread's share of the sequences ----
   const int share = (p.B + kDecThreads - 1) / kDecThreads;
   const int b_lo = min(tid * share, p.B), b_hi = min(b_lo + share, p.B);
   int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += (dec_len(p, b, blockIdx.x == 0) + kTile - 1) / kTile;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int len = dec_len(p, b, blockIdx.x == 0);
+    if (len > 0) mine += (len + kTile - 1) / kTile + kDecItemCost;
+  }
   mine *= items;
   int64_t incl = mine;
 #pragma unroll
@@ -235,11 +245,32 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
     grid_launch_dependents();
     return;
   }
-  auto owner = [&](int64_t t) { return ((t + 1) * ctas - 1) / total; };
+  auto owner = [&](int64_t t) { return static_cast<int>(((t + 1) * ctas - 1) / total); };
 
-  // the tile t0: the thread share it falls in, then along that share
-  DecCursor cur;
-  int64_t item_t0;      // flat index of the current item's first tile
+  auto enter = [&](DecWalk& w) {              // w.b, w.sub and w.start are set
+    w.n = (w.len + kTile - 1) / kTile;
+    const int64_t first = w.start + kDecItemCost;
+    w.j = t0 > first ? static_cast<int>(t0 - first) : 0;
+    w.j_end = t1 - first < w.n ? static_cast<int>(t1 - first) : w.n;
+    w.done = first >= t1;
+  };
+  auto next_item = [&](DecWalk& w) {
+    w.start += w.n + kDecItemCost;
+    if (w.start + kDecItemCost >= t1) {
+      w.done = true;
+      return;
+    }
+    if (++w.sub == items) {
+      w.sub = 0;
+      do {
+        ++w.b;
+        w.len = dec_len(p, w.b, false);
+      } while (w.len == 0);
+    }
+    enter(w);
+  };
+  // the item of t0: the thread share it falls in, then along that share
+  DecWalk cur;
   {
     int lo = 0, hi = kDecThreads - 1;
     while (lo < hi) {
@@ -248,90 +279,93 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
       else hi = mid - 1;
     }
     int64_t at = s_scan[lo];
-    int b = lo * share;
+    int b = lo * share, per = 0;
     for (;; ++b) {
       cur.len = dec_len(p, b, false);
-      cur.n = (cur.len + kTile - 1) / kTile;
-      const int64_t here = static_cast<int64_t>(cur.n) * items;
+      per = cur.len > 0 ? (cur.len + kTile - 1) / kTile + kDecItemCost : 0;
+      const int64_t here = static_cast<int64_t>(per) * items;
       if (t0 < at + here) break;
       at += here;
     }
     cur.b = b;
-    const int64_t in = t0 - at;
-    cur.sub = static_cast<int>(in / cur.n);
-    cur.j = static_cast<int>(in - static_cast<int64_t>(cur.sub) * cur.n);
-    item_t0 = t0 - cur.j;
+    cur.sub = static_cast<int>((t0 - at) / per);
+    cur.start = at + static_cast<int64_t>(cur.sub) * per;
+    enter(cur);
+    if (!cur.done && cur.j >= cur.j_end) cur.done = true;      // (t1 lies before its first tile)
   }
-  auto next_item = [&](DecCursor& c) {
-    c.j = 0;
-    if (++c.sub == items) {
-      c.sub = 0;
-      do {
-        ++c.b;
-        c.len = dec_len(p, c.b, false);
-      } while (c.len == 0);
-      c.n = (c.len + kTile - 1) / kTile;
-    }
-  };
+  if (cur.done) {
+    grid_launch_dependents();
+    return;
+  }
 
   // ---- the copies of a step: page numbers one step ahead of the rows ----
-  constexpr int kIds = (kTok + 31) / 32;     // rows per lane whose pages it looks up
-  DecCursor pre = cur;                       // the next step to look up
-  int64_t pre_t = t0;
-  int id_page[kIds], id_at[kIds], id_head = 0;
-  bool id_ok[kIds];
+  constexpr int kIds = (kTok + 31) / 32;      // rows per lane whose pages it looks up
+  DecWalk pre = cur;                          // the next step to look up
+  int id_page[kIds], id_at[kIds], id_head = 0, id_left = 0;
   auto look_up = [&]() {
-    if (pre_t >= t1) {
-#pragma unroll
-      for (int i = 0; i < kIds; ++i) id_ok[i] = false;
-      return;
-    }
+    id_left = 0;
+    if (pre.done) return;
     id_head = pre.sub / p.blocks;
+    const int base = pre.j * kTile + warp * kTok;
+    id_left = pre.len - base;
 #pragma unroll
     for (int i = 0; i < kIds; ++i) {
       const int r = lane + 32 * i;
-      const int tok = pre.j * kTile + warp * kTok + r;
-      id_ok[i] = r < kTok && tok < pre.len;
-      if (id_ok[i]) {
+      if (r < kTok && r < id_left) {
+        const int tok = base + r;
         const int c = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.cache.page_size;
         id_at[i] = tok - c * p.cache.page_size;
         id_page[i] = __ldg(p.table + pre.b * p.ld_table + c);
       }
     }
-    ++pre_t;
-    if (++pre.j == pre.n && pre_t < t1) next_item(pre);
+    if (++pre.j == pre.j_end) next_item(pre);
   };
+  const int chunk = lane % Cfg::kChunks;
+  const char* k_base = static_cast<const char*>(p.cache.k) + 16 * chunk;
+  const char* v_base = static_cast<const char*>(p.cache.v) + 16 * chunk;
+  const uint32_t k_dst = ring + (lane / Cfg::kChunks) * kRowK + 16 * chunk;
+  const uint32_t v_dst = ring + kTok * kRowK + (lane / Cfg::kChunks) * kRowV + 16 * chunk;
   auto issue = [&](int stage) {
+    constexpr int kUnit = kFp8 ? 16 : 8;       // elements in 16 bytes
+    constexpr int kStep = 32 / Cfg::kChunks;   // rows per copy of the warp
     uint64_t mask = 0;
-    __syncwarp();                            // every lane has read the previous offsets
 #pragma unroll
     for (int i = 0; i < kIds; ++i) {
       const int r = lane + 32 * i;
-      longlong2 off = make_longlong2(-1, -1);
-      if (id_ok[i]) {
-        if (static_cast<unsigned>(id_page[i]) < static_cast<uint64_t>(p.cache.num_pages)) {
-          off.x = (id_page[i] * p.cache.k_page + id_at[i] * p.cache.k_slot + id_head * p.cache.k_head) * (kFp8 ? 1 : 2);
-          off.y = (id_page[i] * p.cache.v_page + id_at[i] * p.cache.v_slot + id_head * p.cache.v_head) * (kFp8 ? 1 : 2);
-        } else {
-          record_error(kSiteBadIndex);
-        }
+      bool ok = r < kTok && r < id_left;
+      if (ok && static_cast<unsigned>(id_page[i]) >= static_cast<uint64_t>(p.cache.num_pages)) {
+        record_error(kSiteBadIndex);
+        ok = false;
       }
-      if (r < kTok) s_off[warp][r] = off;
-      mask |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, off.x >= 0)) << (32 * i);
+      if (r < kTok) {
+        uint2 off = make_uint2(0, 0);
+        if (ok) {
+          off.x = static_cast<uint32_t>((id_page[i] * p.cache.k_page + id_at[i] * p.cache.k_slot + id_head * p.cache.k_head) / kUnit);
+          off.y = static_cast<uint32_t>((id_page[i] * p.cache.v_page + id_at[i] * p.cache.v_slot + id_head * p.cache.v_head) / kUnit);
+        }
+        s_off[warp][r] = off;
+      }
+      mask |= static_cast<uint64_t>(__ballot_sync(0xffffffffu, ok)) << (32 * i);
     }
     if (lane == 0) s_mask[warp][stage] = mask;
     __syncwarp();
-    if (mask) {
-      const uint32_t dst = ring_a + stage * kDecStageBytes;
-      const int c = lane % Cfg::kChunks;
+    const uint2* off = &s_off[warp][lane / Cfg::kChunks];
+    const uint32_t at = stage * Cfg::kStage;
+    if (mask == kFull) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int r = lane / Cfg::kChunks + i * (32 / Cfg::kChunks);
-        const longlong2 off = s_off[warp][r];
-        const uint32_t n = off.x >= 0 ? 16u : 0u;
-        const int64_t ko = off.x >= 0 ? off.x + 16 * c : 0, vo = off.x >= 0 ? off.y + 16 * c : 0;
-        cp_async16(dst + dec_chunk<D, kFp8, false>(r, c), static_cast<const char*>(p.cache.k) + ko, n);
-        cp_async16(dst + kDecStageBytes / 2 + dec_chunk<D, kFp8, true>(r, c), static_cast<const char*>(p.cache.v) + vo, n);
+        const uint2 x = off[i * kStep];
+        cp_async16(k_dst + at + i * kStep * kRowK, k_base + static_cast<uint64_t>(x.x) * 16);
+        cp_async16(v_dst + at + i * kStep * kRowV, v_base + static_cast<uint64_t>(x.y) * 16);
+      }
+    } else if (mask) {
+      // rows that do not count are filled with zeros
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const uint2 x = off[i * kStep];
+        const uint32_t n = (mask >> (lane / Cfg::kChunks + i * kStep)) & 1 ? 16 : 0;
+        cp_async16_or_zero(k_dst + at + i * kStep * kRowK, k_base + static_cast<uint64_t>(x.x) * 16, n);
+        cp_async16_or_zero(v_dst + at + i * kStep * kRowV, v_base + static_cast<uint64_t>(x.y) * 16, n);
       }
     }
     cp_async_commit();
@@ -341,44 +375,62 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
 #pragma unroll
   for (int s = 0; s < kDecStages - 1; ++s) {
     issue(s);
+    __syncwarp();                              // the offsets are read before the next ones
     look_up();
   }
 
+  // q as it lies: lane (g, t4) reads the values of head g that it will hold
+  constexpr int kRaw = kFp8 ? 2 * kKT : 2 * kKT;
+  uint32_t raw[kNT][kRaw];
+  auto fetch_q = [&](const DecWalk& w) {
+    const int hk = w.sub / p.blocks, hb = w.sub - hk * p.blocks;
+    const int h0 = hk * p.group + hb * 8 * kNT;
+    const int heads = min(8 * kNT, p.group - hb * 8 * kNT);
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int h = 8 * nt + g;
+      const __nv_bfloat16* src = p.q + w.b * p.q_token + (h0 + h) * p.q_head;
+      const bool ok = h < heads;
+#pragma unroll
+      for (int k = 0; k < kKT; ++k) {
+        if constexpr (!kFp8) {
+          raw[nt][2 * k] = ok ? __ldg(reinterpret_cast<const unsigned int*>(src + 16 * k + 2 * t4)) : 0u;
+          raw[nt][2 * k + 1] = ok ? __ldg(reinterpret_cast<const unsigned int*>(src + 16 * k + 8 + 2 * t4)) : 0u;
+        } else {
+          const uint2 x = ok ? __ldg(reinterpret_cast<const uint2*>(src + 16 * (t4 + 4 * (k / 4)) + 4 * (k % 4))) : make_uint2(0, 0);
+          raw[nt][2 * k] = x.x;
+          raw[nt][2 * k + 1] = x.y;
+        }
+      }
+    }
+  };
+  fetch_q(cur);
+
   int stage = 0;
-  int64_t t = t0;
-  while (t < t1) {
-    const int64_t seg = (cur.n - cur.j) < (t1 - t) ? (cur.n - cur.j) : (t1 - t);
+  while (!cur.done) {
     const int hk = cur.sub / p.blocks, hb = cur.sub - hk * p.blocks;
     const int h0 = hk * p.group + hb * 8 * kNT;            // first query head
     const int heads = min(8 * kNT, p.group - hb * 8 * kNT);
 
-    // q as the B operand: lane (g, t4) holds head g's values.  bf16: as they
-    // lie.  e4m3 cache: f16, scaled by a power of two so that the largest is
-    // in [1, 2) (exact; what falls below 2^-24 of it is lost), k steps in the
-    // order of the k rows' 16-byte chunks.
+    // q as the B operand.  bf16: as it lies.  e4m3 cache: f16, scaled by a
+    // power of two so that a head's largest is in [1, 2) (exact; what falls
+    // below 2^-24 of it is lost), k steps in the order of the k rows' 16-byte
+    // chunks.
     uint32_t qf[kNT][kKT][2];
     float sc[kNT][2];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      const int h = 8 * nt + g;
-      const __nv_bfloat16* src = p.q + cur.b * p.q_token + (h0 + h) * p.q_head;
-      const bool ok = h < heads;
       if constexpr (!kFp8) {
 #pragma unroll
         for (int k = 0; k < kKT; ++k) {
-          qf[nt][k][0] = ok ? __ldg(reinterpret_cast<const unsigned int*>(src + 16 * k + 2 * t4)) : 0u;
-          qf[nt][k][1] = ok ? __ldg(reinterpret_cast<const unsigned int*>(src + 16 * k + 8 + 2 * t4)) : 0u;
+          qf[nt][k][0] = raw[nt][2 * k];
+          qf[nt][k][1] = raw[nt][2 * k + 1];
         }
         sc[nt][0] = sc[nt][1] = p.scale_log2;
       } else {
         float amax = 0.0f;
-        uint2 raw[kKT];
 #pragma unroll
-        for (int k = 0; k < kKT; ++k) {
-          raw[k] = ok ? __ldg(reinterpret_cast<const uint2*>(src + 16 * (t4 + 4 * (k / 4)) + 4 * (k % 4))) : make_uint2(0, 0);
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(raw[k].x)), fabsf(bf16_hi(raw[k].x))),
-                                   fmaxf(fabsf(bf16_lo(raw[k].y)), fabsf(bf16_hi(raw[k].y)))));
-        }
+        for (int k = 0; k < kRaw; ++k) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(raw[nt][k])), fabsf(bf16_hi(raw[nt][k]))));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         // 2^e <= amax < 2^(e+1); e from the exponent field, kept where 2^-e is normal too
@@ -386,8 +438,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
         for (int k = 0; k < kKT; ++k) {
-          qf[nt][k][0] = pack2<true>(bf16_lo(raw[k].x) * down, bf16_hi(raw[k].x) * down);
-          qf[nt][k][1] = pack2<true>(bf16_lo(raw[k].y) * down, bf16_hi(raw[k].y) * down);
+          qf[nt][k][0] = pack2<true>(bf16_lo(raw[nt][2 * k]) * down, bf16_hi(raw[nt][2 * k]) * down);
+          qf[nt][k][1] = pack2<true>(bf16_lo(raw[nt][2 * k + 1]) * down, bf16_hi(raw[nt][2 * k + 1]) * down);
         }
         const float up = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
         sc[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t4);
@@ -403,16 +455,16 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
       for (int i = 0; i < kMT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
     }
 
-    for (int64_t step = 0; step < seg; ++step) {
+    for (int j = cur.j; j < cur.j_end; ++j) {
       cp_async_wait<kDecStages - 2>();
       __syncwarp();
       {
-        int ahead = stage + kDecStages - 1;
+        int ahead = stage + kDecStages - 1;    // the stage that the step before has left
         if (ahead >= kDecStages) ahead -= kDecStages;
         issue(ahead);
         look_up();
       }
-      const uint32_t ka = ring_a + stage * kDecStageBytes, va = ka + kDecStageBytes / 2;
+      const uint32_t ka = ring + stage * Cfg::kStage, va = ka + kTok * kRowK;
       const uint64_t mask = s_mask[warp][stage];
       if (++stage == kDecStages) stage = 0;
       if (mask == 0) continue;
@@ -420,21 +472,26 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
       float s[kNT][kTT][4];
 #pragma unroll
       for (int tt = 0; tt < kTT; ++tt) {
+        float s2[kNT][4];                      // two chains of products
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) s[nt][tt][0] = s[nt][tt][1] = s[nt][tt][2] = s[nt][tt][3] = 0.0f;
+        for (int nt = 0; nt < kNT; ++nt) {
+          s[nt][tt][0] = s[nt][tt][1] = s[nt][tt][2] = s[nt][tt][3] = 0.0f;
+          s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.0f;
+        }
         if constexpr (!kFp8) {
+          const uint32_t at = ka + (16 * tt + (lane & 15)) * kRowK + (lane >> 4) * 16;
 #pragma unroll
           for (int k = 0; k < kKT; ++k) {
             uint32_t a[4];
-            ldsm4(a, ka + dec_chunk<D, kFp8, false>(16 * tt + (lane & 15), 2 * k + (lane >> 4)));
+            ldsm4(a, at + 32 * k);
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) mma16816<false>(s[nt][tt], a, qf[nt][k][0], qf[nt][k][1]);
+            for (int nt = 0; nt < kNT; ++nt) mma16816<false>((k & 1) ? s2[nt] : s[nt][tt], a, qf[nt][k][0], qf[nt][k][1]);
           }
         } else {
+          const uint32_t at = ka + (16 * tt + g) * kRowK + t4 * 16;
 #pragma unroll
           for (int c = 0; c < D / 64; ++c) {
-            const uint4 r0 = lds128(ka + dec_chunk<D, kFp8, false>(16 * tt + g, t4 + 4 * c));
-            const uint4 r1 = lds128(ka + dec_chunk<D, kFp8, false>(16 * tt + g + 8, t4 + 4 * c));
+            const uint4 r0 = lds128(at + 64 * c), r1 = lds128(at + 8 * kRowK + 64 * c);
             const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -442,27 +499,32 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
                                      e4m3x2_to_f16x2(static_cast<uint16_t>(w0[k] >> 16)),
                                      e4m3x2_to_f16x2(static_cast<uint16_t>(w1[k] >> 16))};
 #pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) mma16816<true>(s[nt][tt], a, qf[nt][4 * c + k][0], qf[nt][4 * c + k][1]);
+              for (int nt = 0; nt < kNT; ++nt)
+                mma16816<true>((k & 1) ? s2[nt] : s[nt][tt], a, qf[nt][4 * c + k][0], qf[nt][4 * c + k][1]);
             }
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[nt][tt][i] = (s[nt][tt][i] + s2[nt][i]) * sc[nt][i & 1];
       }
       // ---- softmax ----
-      const bool full = kTok == 64 ? mask == ~0ull : mask == (1ull << (kTok & 63)) - 1;
+      if (mask != kFull) {
+#pragma unroll
+        for (int tt = 0; tt < kTT; ++tt)
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            if (!((mask >> (16 * tt + g)) & 1)) s[nt][tt][0] = s[nt][tt][1] = -INFINITY;
+            if (!((mask >> (16 * tt + g + 8)) & 1)) s[nt][tt][2] = s[nt][tt][3] = -INFINITY;
+          }
+      }
       uint32_t pf[kNT][kTT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
         float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int tt = 0; tt < kTT; ++tt) {
-          s[nt][tt][0] *= sc[nt][0];
-          s[nt][tt][1] *= sc[nt][1];
-          s[nt][tt][2] *= sc[nt][0];
-          s[nt][tt][3] *= sc[nt][1];
-          if (!full) {
-            if (!((mask >> (16 * tt + g)) & 1)) s[nt][tt][0] = s[nt][tt][1] = -INFINITY;
-            if (!((mask >> (16 * tt + g + 8)) & 1)) s[nt][tt][2] = s[nt][tt][3] = -INFINITY;
-          }
           mx0 = fmaxf(mx0, fmaxf(s[nt][tt][0], s[nt][tt][2]));
           mx1 = fmaxf(mx1, fmaxf(s[nt][tt][1], s[nt][tt][3]));
         }
@@ -471,9 +533,9 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
           mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
         }
-        mx0 = fmaxf(mx0, m[nt][0]);
-        mx1 = fmaxf(mx1, m[nt][1]);
         if (__any_sync(0xffffffffu, mx0 > m[nt][0] || mx1 > m[nt][1])) {
+          mx0 = fmaxf(mx0, m[nt][0]);
+          mx1 = fmaxf(mx1, m[nt][1]);
           const float a0 = m[nt][0] == -INFINITY ? 0.0f : ex2(m[nt][0] - mx0);
           const float a1 = m[nt][1] == -INFINITY ? 0.0f : ex2(m[nt][1] - mx1);
           m[nt][0] = mx0;
@@ -505,10 +567,11 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
 #pragma unroll
       for (int tt = 0; tt < kTT; ++tt) {
         if constexpr (!kFp8) {
+          const uint32_t at = va + (16 * tt + (lane & 7) + ((lane >> 4) << 3)) * kRowV + ((lane >> 3) & 1) * 16;
 #pragma unroll
           for (int i = 0; i < kMT; ++i) {
             uint32_t a[4];
-            ldsm4_t(a, va + dec_chunk<D, kFp8, true>(16 * tt + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+            ldsm4_t(a, at + 32 * i);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) mma16816<false>(o[nt][i], a, pf[nt][tt][0], pf[nt][tt][1]);
           }
@@ -516,17 +579,18 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
           // lane (g, t4) holds bytes g D/8 .. of tokens 2 t4, 2 t4 + 1, 2 t4 + 8,
           // 2 t4 + 9; row g of the i-th product is value g D/8 + 2 i, row g + 8 the next
           uint32_t w[4][D / 32];
+          const uint32_t at = va + (16 * tt + 2 * t4) * kRowV + g * (D / 8);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int row = 16 * tt + 2 * t4 + (r & 1) + ((r >> 1) << 3);
+            const uint32_t row = at + ((r & 1) + ((r >> 1) << 3)) * kRowV;
             if constexpr (D == 128) {
-              const uint4 x = lds128(va + dec_chunk<D, kFp8, true>(row, g));
+              const uint4 x = lds128(row);
               w[r][0] = x.x;
               w[r][1] = x.y;
               w[r][2] = x.z;
               w[r][3] = x.w;
             } else {
-              const uint2 x = lds64(va + dec_chunk<D, kFp8, true>(row, g >> 1) + 8 * (g & 1));
+              const uint2 x = lds64(row);
               w[r][0] = x.x;
               w[r][1] = x.y;
             }
@@ -545,10 +609,13 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
       }
     }
 
-    // ---- the segment's result: the four warps joined, 4 heads at a time ----
-    const int64_t first = owner(item_t0), last = owner(item_t0 + cur.n - 1);
+    // ---- the item's result: the four warps joined, 2 heads at a time ----
+    const int first = owner(cur.start + kDecItemCost), last = owner(cur.start + kDecItemCost + cur.n - 1);
     const bool whole = first == last;
+    const int b = cur.b;
     float* slot = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == first ? 1 : 0)) * kSlot;
+    next_item(cur);
+    if (!cur.done) fetch_q(cur);               // arrives meanwhile
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
@@ -557,13 +624,11 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
         l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], x);
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int h4 = 8 * nt + 4 * half;                  // heads h4 .. h4 + n4
-        const int n4 = min(4, heads - h4);
-        if (n4 <= 0) break;
-        if ((t4 >> 1) == half) {
-          const int h = 2 * (t4 & 1);
-          float* so = s_o + (warp * 4 + h) * Cfg::kPad;
+      for (int q = 0; q < 4; ++q) {
+        const int h2 = 8 * nt + 2 * q;                     // heads h2, h2 + 1
+        if (h2 >= heads) break;
+        if (t4 == q) {
+          float* so = s_o + warp * 2 * Cfg::kPad;
 #pragma unroll
           for (int i = 0; i < kMT; ++i) {
             const int d0 = kFp8 ? g * (D / 8) + 2 * i : 16 * i + g;
@@ -574,15 +639,16 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
             so[Cfg::kPad + d1] = o[nt][i][3];
           }
           if (g == 0) {
-            s_m[warp][h] = m[nt][0];
-            s_m[warp][h + 1] = m[nt][1];
-            s_l[warp][h] = l[nt][0];
-            s_l[warp][h + 1] = l[nt][1];
+            s_m[warp][0] = m[nt][0];
+            s_m[warp][1] = m[nt][1];
+            s_l[warp][0] = l[nt][0];
+            s_l[warp][1] = l[nt][1];
           }
         }
         __syncthreads();
-        for (int i = tid; i < n4 * (D / 4); i += kDecThreads) {
+        for (int i = tid; i < 2 * (D / 4); i += kDecThreads) {
           const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+          if (h2 + h >= heads) break;
           float mm = s_m[0][h];
 #pragma unroll
           for (int w = 1; w < kDecWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
@@ -591,7 +657,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
 #pragma unroll
           for (int w = 0; w < kDecWarps; ++w) {
             const float a = s_m[w][h] == -INFINITY ? 0.0f : ex2(s_m[w][h] - mm);
-            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 4 + h) * Cfg::kPad + d);
+            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 2 + h) * Cfg::kPad + d);
             ll += a * s_l[w][h];
             v.x += a * x.x;
             v.y += a * x.y;
@@ -599,12 +665,12 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
             v.w += a * x.w;
           }
           if (whole) {
-            dec_store<D>(p, cur.b, h0 + h4 + h, d, v, mm, ll);
+            dec_store<D>(p, b, h0 + h2 + h, d, v, mm, ll);
           } else {
-            *reinterpret_cast<float4*>(slot + (h4 + h) * D + d) = v;
+            *reinterpret_cast<float4*>(slot + (h2 + h) * D + d) = v;
             if (d == 0) {
-              slot[8 * kNT * D + h4 + h] = mm;
-              slot[8 * kNT * (D + 1) + h4 + h] = ll;
+              slot[8 * kNT * D + h2 + h] = mm;
+              slot[8 * kNT * (D + 1) + h2 + h] = ll;
             }
           }
         }
@@ -621,7 +687,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
         // ranges w, w + 4, ...; then the warps in order
         __threadfence();
         if (tid == 0) p.counters[first] = 0;
-        const int n = static_cast<int>(last - first) + 1;
+        const int n = last - first + 1;
         auto part = [&](int i) {
           return p.partials + (static_cast<int64_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * kSlot;
         };
@@ -665,15 +731,12 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
               v.z += x.z;
               v.w += x.w;
             }
-            dec_store<D>(p, cur.b, h0 + hh, d, v, mm, ll);
+            dec_store<D>(p, b, h0 + hh, d, v, mm, ll);
           }
           __syncthreads();
         }
       }
     }
-    t += seg;
-    item_t0 += cur.n;
-    if (t < t1) next_item(cur);
   }
   cp_async_wait<0>();
   grid_launch_dependents();

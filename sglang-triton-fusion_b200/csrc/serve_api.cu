@@ -229,6 +229,13 @@ int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t 
   p.Hq = Hq;
   p.Hkv = Hkv;
   const bool fp8 = cache->dtype == FP8GQ_DTYPE_E4M3;
+  // rows are addressed by 32-bit offsets in units of 16 bytes
+  for (int kv = 0; kv < 2; ++kv) {
+    const int64_t span = (cache->num_pages - 1) * (kv ? cache->v_page_stride : cache->k_page_stride) +
+                         (cache->page_size - 1) * (kv ? cache->v_slot_stride : cache->k_slot_stride) +
+                         (Hkv - 1) * (kv ? cache->v_head_stride : cache->k_head_stride) + D;
+    if (span / (fp8 ? 16 : 8) > UINT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
+  }
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (cache->page_size == 1 << i) p.page_shift = i;
