@@ -135,6 +135,12 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
+// Two e4m3 codes -> two f16 values (exact).
+__device__ __forceinline__ uint32_t cvt_e4m3x2(uint16_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
+  return r;
+}
 template <bool kF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (kF16) {
@@ -157,15 +163,16 @@ __device__ __forceinline__ int dec_len(const DecodeParams& p, int b, bool record
   return n;
 }
 
-// Four values of head h's output from their sum v and the weights' sum l
-// (relative to the maximum m); l = 0 where no token counted.
-template <int D>
-__device__ __forceinline__ void dec_store(const DecodeParams& p, int b, int h, int d, float4 v, float m, float l) {
+// N values of head h's output from their sum v and the weights' sum l (relative
+// to the maximum m); l = 0 where no token counted.
+template <int N>
+__device__ __forceinline__ void dec_store(const DecodeParams& p, int b, int h, int d, const float (&v)[N], float m, float l) {
   const float r = l > 0.0f ? p.out_scale / l : l;      // NaN stays
-  uint2 w;
-  w.x = pack2<false>(v.x * r, v.y * r);
-  w.y = pack2<false>(v.z * r, v.w * r);
-  *reinterpret_cast<uint2*>(p.out + b * p.o_token + h * p.o_head + d) = w;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + b * p.o_token + h * p.o_head + d);
+  if constexpr (N == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<false>(v[0] * r, v[1] * r), pack2<false>(v[2] * r, v[3] * r));
+  else
+    *dst = pack2<false>(v[0] * r, v[1] * r);
   if (p.lse && d == 0)
     p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
@@ -495,9 +502,9 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
             const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint32_t a[4] = {e4m3x2_to_f16x2(static_cast<uint16_t>(w0[k])), e4m3x2_to_f16x2(static_cast<uint16_t>(w1[k])),
-                                     e4m3x2_to_f16x2(static_cast<uint16_t>(w0[k] >> 16)),
-                                     e4m3x2_to_f16x2(static_cast<uint16_t>(w1[k] >> 16))};
+              const uint32_t a[4] = {cvt_e4m3x2(static_cast<uint16_t>(w0[k])), cvt_e4m3x2(static_cast<uint16_t>(w1[k])),
+                                     cvt_e4m3x2(static_cast<uint16_t>(w0[k] >> 16)),
+                                     cvt_e4m3x2(static_cast<uint16_t>(w1[k] >> 16))};
 #pragma unroll
               for (int nt = 0; nt < kNT; ++nt)
                 mma16816<true>((k & 1) ? s2[nt] : s[nt][tt], a, qf[nt][4 * c + k][0], qf[nt][4 * c + k][1]);
@@ -600,8 +607,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
             const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;     // bytes 2i, 2i + 1 of both tokens, paired by byte
             const uint32_t lo = __byte_perm(w[0][i >> 1], w[1][i >> 1], sel);
             const uint32_t hi = __byte_perm(w[2][i >> 1], w[3][i >> 1], sel);
-            const uint32_t a[4] = {e4m3x2_to_f16x2(static_cast<uint16_t>(lo)), e4m3x2_to_f16x2(static_cast<uint16_t>(lo >> 16)),
-                                   e4m3x2_to_f16x2(static_cast<uint16_t>(hi)), e4m3x2_to_f16x2(static_cast<uint16_t>(hi >> 16))};
+            const uint32_t a[4] = {cvt_e4m3x2(static_cast<uint16_t>(lo)), cvt_e4m3x2(static_cast<uint16_t>(lo >> 16)),
+                                   cvt_e4m3x2(static_cast<uint16_t>(hi)), cvt_e4m3x2(static_cast<uint16_t>(hi >> 16))};
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) mma16816<true>(o[nt][i], a, pf[nt][tt][0], pf[nt][tt][1]);
           }
@@ -665,7 +672,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
             v.w += a * x.w;
           }
           if (whole) {
-            dec_store<D>(p, b, h0 + h2 + h, d, v, mm, ll);
+            const float o4[4] = {v.x, v.y, v.z, v.w};
+            dec_store<4>(p, b, h0 + h2 + h, d, o4, mm, ll);
           } else {
             *reinterpret_cast<float4*>(slot + (h2 + h) * D + d) = v;
             if (d == 0) {
@@ -683,57 +691,64 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
       if (tid == 0) s_last = atomic_add_acq_rel_gpu(p.counters + first, 1) == last - first;
       __syncthreads();
       if (s_last) {
-        // join the ranges' partial results in range order: warp w takes
-        // ranges w, w + 4, ...; then the warps in order
+        // join the ranges' partial results in range order: a warp per head, its
+        // lanes over the head's values
         __threadfence();
         if (tid == 0) p.counters[first] = 0;
         const int n = last - first + 1;
         auto part = [&](int i) {
           return p.partials + (static_cast<int64_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * kSlot;
         };
-        constexpr int kLanes = D / 4;            // lanes per head
-        constexpr int kPer = 32 / kLanes;        // heads at once
-        for (int hh0 = 0; hh0 < heads; hh0 += kPer) {
-          const int hh = hh0 + lane / kLanes, d = (lane % kLanes) * 4;
-          const bool ok = hh < heads;
-          float mm = -INFINITY;
-          for (int i = lane % kLanes; ok && i < n; i += kLanes) mm = fmaxf(mm, __ldcg(part(i) + 8 * kNT * D + hh));
+        for (int h = warp; h < heads; h += kDecWarps) {
+          constexpr int kAhead = 8;
+          constexpr int kPer = D / 32;           // values per lane
+          float v[kPer] = {}, mm = -INFINITY, ll = 0.0f;
+          for (int i0 = 0; i0 < n; i0 += 32) {
+            // lane i: range i0 + i
+            const int k = min(32, n - i0);
+            const float mi = lane < k ? __ldcg(part(i0 + lane) + 8 * kNT * D + h) : -INFINITY;
+            const float li = lane < k ? __ldcg(part(i0 + lane) + 8 * kNT * (D + 1) + h) : 0.0f;
+            float mx = mi;
 #pragma unroll
-          for (int x = kLanes / 2; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-          float ll = 0.0f;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (ok) {
-#pragma unroll 4
-            for (int i = warp; i < n; i += kDecWarps) {
-              const float* q = part(i);
-              const float mi = __ldcg(q + 8 * kNT * D + hh), li = __ldcg(q + 8 * kNT * (D + 1) + hh);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(q + hh * D + d));
-              const float a = mi == -INFINITY ? 0.0f : ex2(mi - mm);
-              ll += a * li;
-              v.x += a * x.x;
-              v.y += a * x.y;
-              v.z += a * x.z;
-              v.w += a * x.w;
-            }
-            *reinterpret_cast<float4*>(s_o + (warp * kPer + lane / kLanes) * D + d) = v;
-            if (d == 0) s_l[warp][lane / kLanes] = ll;
-          }
-          __syncthreads();
-          if (warp == 0 && ok) {
-            ll = 0.0f;
-            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            mx = fmaxf(mx, mm);
+            const float old = mm == -INFINITY ? 0.0f : ex2(mm - mx);
+            const float a = mi == -INFINITY ? 0.0f : ex2(mi - mx);
+            float sum = a * li;
 #pragma unroll
-            for (int w = 0; w < kDecWarps; ++w) {
-              const float4 x = *reinterpret_cast<const float4*>(s_o + (w * kPer + lane / kLanes) * D + d);
-              ll += s_l[w][lane / kLanes];
-              v.x += x.x;
-              v.y += x.y;
-              v.z += x.z;
-              v.w += x.w;
+            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            ll = ll * old + sum;
+            mm = mx;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[e] *= old;
+            for (int i = 0; i < k; i += kAhead) {
+              float x[kAhead][kPer];
+#pragma unroll
+              for (int u = 0; u < kAhead; ++u)
+                if (i + u < k) {
+                  const float* src = part(i0 + i + u) + h * D + kPer * lane;
+                  if constexpr (kPer == 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+                    x[u][0] = y.x;
+                    x[u][1] = y.y;
+                    x[u][2] = y.z;
+                    x[u][3] = y.w;
+                  } else {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+                    x[u][0] = y.x;
+                    x[u][1] = y.y;
+                  }
+                }
+#pragma unroll
+              for (int u = 0; u < kAhead; ++u) {
+                const float f = __shfl_sync(0xffffffffu, a, (i + u) & 31);
+                if (i + u < k)
+#pragma unroll
+                  for (int e = 0; e < kPer; ++e) v[e] = __fmaf_rn(f, x[u][e], v[e]);
+              }
             }
-            dec_store<D>(p, b, h0 + hh, d, v, mm, ll);
           }
-          __syncthreads();
+          dec_store<kPer>(p, b, h0 + h, kPer * lane, v, mm, ll);
         }
       }
     }
