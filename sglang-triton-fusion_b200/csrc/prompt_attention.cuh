@@ -4,23 +4,26 @@
 // running maximum m and sum l of the softmax; O is rescaled when m moves.
 //
 // Bound: the tensor cores (4 D flops per visible pair and head) and, next to
-// them, the exponentials: 128 x 128 of a tile take the MUFU as long as the
-// tile's two products take the tensor core.  So a CTA carries two query tiles
-// in turn: while one tile's scores are in the softmax, the other's products
-// run.
+// them, the exponentials: those of a tile keep the MUFU as busy as its two
+// products keep the tensor core.  So a CTA carries two query tiles, each with
+// its own softmax warps and MMA warp, that run past each other freely.
 //
 // Query tile: 128 rows = R tokens x the G query heads of one kv head (R = 128 /
 // G), loaded by one box [R][G][64] per half head, so that k and v are read once
 // for the whole group, short prompts fill the tile, and a causal tile spans few
-// tokens.  k and v tiles (128 tokens) go through a ring of shared-memory slots
-// filled by TMA.  Scores and outputs live in TMEM (S0, S1, O0, O1); the weights
-// P overwrite their scores as bf16 and are the A operand of the second product
-// straight from TMEM; v is read as it lies (its N side contiguous).
+// tokens.  k and v tiles (kKeys tokens) go through a ring of shared-memory slots
+// filled by TMA.  TMEM holds, for each query tile, the scores S, the weights P
+// (bf16, the A operand of the second product straight from TMEM) and O.  P has
+// columns of its own, so that the next scores are computed while the softmax
+// works on these; that is what sets kKeys: 80 keys at D = 128 (S 80 + P 40 + O
+// 128 columns, twice, of 512), 128 at D = 64.  With 128 keys and P over S at
+// D = 128, the softmax waited 1900 of 4100 cycles a tile for the products and
+// 8192 tokens took 607 us.  v is read as it lies (its N side contiguous).
 //
 // Warps 0-3 and 4-7: softmax, output (one thread per row of tile 0, 1).  Warp 8:
 // TMA; it also clears the rows of the last v tile that lie past the sequence
 // (another sequence's values, which a weight of 0 does not stop if they are
-// NaN).  Warp 9: MMA.
+// NaN).  Warps 9, 10: MMA of tile 0, 1.
 #pragma once
 
 #include "fp8gq_device.cuh"
@@ -42,14 +45,19 @@ struct PromptParams {
 };
 
 constexpr int kPrThreads = 384;
-constexpr int kPrKeys = 128;          // keys per tile
 
 template <int D>
 struct PrCfg {
   static constexpr int kHalves = D / 64;
-  static constexpr int kTile = kHalves * 128 * 128;        // bytes of a q, k or v tile
-  static constexpr int kSlots = D == 128 ? 5 : 8;          // ring slots: k and v tiles in turn
-  static constexpr size_t kSmem = 1024 + (2 + kSlots) * static_cast<size_t>(kTile);
+  static constexpr int kKeys = D == 128 ? 80 : 128;        // keys per tile
+  static constexpr int kQTile = kHalves * 128 * 128;       // bytes of a q tile
+  static constexpr int kHalf = kKeys * 128;                // bytes of half a k or v tile (64 values)
+  static constexpr int kTile = kHalves * kHalf;
+  static constexpr int kSlots = 8;                         // ring slots: k and v tiles in turn
+  static constexpr size_t kSmem = 1024 + 2 * static_cast<size_t>(kQTile) + kSlots * static_cast<size_t>(kTile);
+  // TMEM columns: O0 O1 S0 S1 P0 P1
+  static constexpr int kS = 2 * D, kP = kS + 2 * kKeys, kPCols = (kKeys / 2 + 15) / 16 * 16;
+  static_assert(kP + 2 * kPCols <= 512, "TMEM");
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -87,22 +95,17 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 #define FP8GQ_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
 #define FP8GQ_I8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
 
-// 32 columns of this warp's 32 lanes; the registers are valid after tmem_wait_ld.
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+// Columns of this warp's 32 lanes.  Loaded registers are valid after
+// tmem_wait_ld; tmem_loaded keeps their use behind it.
+__device__ __forceinline__ void tmem_ld16r(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : FP8GQ_R8(r, 0), FP8GQ_R8(r, 8), FP8GQ_R8(r, 16), FP8GQ_R8(r, 24)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : FP8GQ_R8(r, 0), FP8GQ_R8(r, 8)
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::FP8GQ_I8(r, 0),
-      FP8GQ_I8(r, 8), FP8GQ_I8(r, 16), FP8GQ_I8(r, 24), "r"(addr)
-      : "memory");
-}
+#define FP8GQ_B8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
+__device__ __forceinline__ void tmem_loaded16(uint32_t* r) { asm volatile("" : FP8GQ_B8(r, 0), FP8GQ_B8(r, 8)::"memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -110,10 +113,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
       FP8GQ_I8(r, 8), "r"(addr)
       : "memory");
 }
-// Keeps the use of registers that tmem_ld32 fills behind tmem_wait_ld.
-#define FP8GQ_B8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
-__device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
-  asm volatile("" : FP8GQ_B8(r, 0), FP8GQ_B8(r, 8), FP8GQ_B8(r, 16), FP8GQ_B8(r, 24)::"memory");
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::FP8GQ_I8(r, 0), "r"(addr)
+               : "memory");
 }
 #undef FP8GQ_B8
 #undef FP8GQ_R8
@@ -140,7 +142,7 @@ __device__ __forceinline__ int pr_cut(int x, int hi) {
 struct PrWork {
   int q0, q1, k0, k1;       // the sequence's tokens
   int r0;                   // first token of the CTA within the sequence
-  int n;                    // key tiles the last row sees
+  int n[2];                 // key tiles that the last row of each query tile sees
 };
 
 template <int D>
@@ -149,15 +151,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
                                                                           const __grid_constant__ CUtensorMap tv,
                                                                           const PromptParams p) {
   using Cfg = PrCfg<D>;
-  constexpr int kSlots = Cfg::kSlots, kTile = Cfg::kTile;
+  constexpr int kSlots = Cfg::kSlots, kTile = Cfg::kTile, kKeys = Cfg::kKeys;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t b_q, b_full[kSlots], b_free[kSlots], b_s[2], b_p[2], b_o, b_fix;
+  __shared__ uint64_t b_q, b_fix;                        // q is there; the last v tile is cleared
+  __shared__ uint64_t b_full[kSlots], b_free[kSlots];
+  __shared__ uint64_t b_s[2], b_r[2], b_p[2], b_o[2];    // scores ready, read; weights ready; O updated
   __shared__ uint32_t s_tmem;
   __shared__ int s_scan[kPrThreads / 32];
   __shared__ PrWork s_work;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t ring = base + 2 * kTile;
+  const uint32_t ring = base + 2 * Cfg::kQTile;
 
   if (warp == 8) {
     if (lane == 0) {
@@ -165,16 +169,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       prefetch_tensormap(&tk);
       prefetch_tensormap(&tv);
       mbar_init(&b_q, 1);
+      mbar_init(&b_fix, 32);
       for (int i = 0; i < kSlots; ++i) {
         mbar_init(&b_full[i], 1);
-        mbar_init(&b_free[i], 1);
+        mbar_init(&b_free[i], 2);         // both MMA warps
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&b_s[i], 1);
-        mbar_init(&b_p[i], 128);
+        mbar_init(&b_r[i], 4);            // softmax warps
+        mbar_init(&b_p[i], 4);
+        mbar_init(&b_o[i], 1);
       }
-      mbar_init(&b_o, 1);
-      mbar_init(&b_fix, 32);
       fence_mbar_init();
     }
   } else if (warp == 9) {
@@ -230,9 +235,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         }
         w.r0 = (nb - 1 - (tile - at)) * span;
         const int lq = w.q1 - w.q0, lk = w.k1 - w.k0;
-        int seen = lk;
-        if (p.causal) seen = min(lk, max(0, min(w.r0 + span, lq) + lk - lq));
-        w.n = (seen + kPrKeys - 1) / kPrKeys;
+        for (int i = 0; i < 2; ++i) {
+          const int end = min(w.r0 + (i + 1) * p.rows, lq);       // past the tile's last token
+          int seen = end > w.r0 + i * p.rows ? lk : 0;
+          if (p.causal && seen) seen = min(lk, max(0, end + lk - lq));
+          w.n[i] = (seen + kKeys - 1) / kKeys;
+        }
         s_work = w;
         break;
       }
@@ -244,219 +252,241 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
   const uint32_t tmem = s_tmem;
   const PrWork w = s_work;
   const int lq = w.q1 - w.q0, lk = w.k1 - w.k0;
-  const bool partial = w.n * kPrKeys > lk;       // the last tile reaches past the sequence
+  const int n = max(w.n[0], w.n[1]);
+  const bool partial = n * kKeys > lk;           // the last tile reaches past the sequence
   bool ok = true;
 
-  if (w.q0 >= 0) {
-    if (warp == 8) {
-      // ---- TMA ----
-      if (lane == 0 && w.n > 0) {
-        mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
-        for (int i = 0; i < 2; ++i)
-          for (int h = 0; h < Cfg::kHalves; ++h)
-            tma_load_3d(base + i * kTile + h * 16384, &tq, 64 * h, hk * p.group, w.q0 + w.r0 + i * p.rows, &b_q);
-        int slot = 0, round = 0, issued = 0;
-        for (int i = 0; i < 2 * w.n && ok; ++i) {      // k and v tiles in turn
-          if (round > 0) ok = mbar_wait(&b_free[slot], (round - 1) & 1, kSitePrompt);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&b_full[slot], kTile);
-          for (int h = 0; h < Cfg::kHalves; ++h)
-            tma_load_3d(ring + slot * kTile + h * 16384, (i & 1) ? &tv : &tk, 64 * h, hk, w.k0 + (i >> 1) * kPrKeys,
-                        &b_full[slot]);
-          ++issued;
-          if (++slot == kSlots) {
-            slot = 0;
-            ++round;
-          }
-        }
-        if (!ok) {
-          // gave up: let the copies in flight land before the CTA may end
-          mbar_wait(&b_q, 0, kSitePrompt);
-          for (int i = issued > kSlots ? issued - kSlots : 0; i < issued; ++i)
-            mbar_wait(&b_full[i % kSlots], (i / kSlots) & 1, kSitePrompt);
+  if (w.q0 >= 0 && n > 0 && warp == 8) {
+    // ---- TMA ----
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
+      for (int i = 0; i < 2; ++i)
+        for (int h = 0; h < Cfg::kHalves; ++h)
+          tma_load_3d(base + i * Cfg::kQTile + h * 16384, &tq, 64 * h, hk * p.group, w.q0 + w.r0 + i * p.rows, &b_q);
+      int slot = 0, round = 0, issued = 0;
+      for (int i = 0; i < 2 * n && ok; ++i) {            // k and v tiles in turn
+        if (round > 0) ok = mbar_wait(&b_free[slot], (round - 1) & 1, kSitePrompt);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&b_full[slot], kTile);
+        for (int h = 0; h < Cfg::kHalves; ++h)
+          tma_load_3d(ring + slot * kTile + h * Cfg::kHalf, (i & 1) ? &tv : &tk, 64 * h, hk, w.k0 + (i >> 1) * kKeys,
+                      &b_full[slot]);
+        ++issued;
+        if (++slot == kSlots) {
+          slot = 0;
+          ++round;
         }
       }
-      // the last v tile's rows past the sequence: zeros
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      if (ok && w.n > 0 && partial) {
-        const int i = 2 * w.n - 1, slot = i % kSlots;
-        if (mbar_wait_warp(&b_full[slot], (i / kSlots) & 1, kSitePrompt, lane)) {
-          const int valid = lk - (w.n - 1) * kPrKeys;
-          const uint32_t v = ring + slot * kTile;
-          for (int x = valid * 8 + lane; x < kPrKeys * 8; x += 32)
-            for (int h = 0; h < Cfg::kHalves; ++h)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * 16384 + x * 16), "r"(0u) : "memory");
-          fence_proxy_async_smem();
-          mbar_arrive(&b_fix);
-        }
+      if (!ok) {
+        // gave up: let the copies in flight land before the CTA may end
+        mbar_wait(&b_q, 0, kSitePrompt);
+        for (int i = issued > kSlots ? issued - kSlots : 0; i < issued; ++i)
+          mbar_wait(&b_full[i % kSlots], (i / kSlots) & 1, kSitePrompt);
       }
-    } else if (warp == 9) {
-      // ---- MMA ----
-      if (lane == 0 && w.n > 0) {
-        const uint32_t id_s = pr_idesc(kPrKeys, false, p.negate != 0), id_o = pr_idesc(D, true, false);
-        int slot = 0, round = 0;
-        auto next = [&]() {
-          if (++slot == kSlots) {
-            slot = 0;
-            ++round;
-          }
-        };
-        auto scores = [&](int i, int at) {
-          const uint32_t a = base + i * kTile, b = ring + at * kTile;
+    }
+    // the last v tile's rows past the sequence: zeros
+    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    if (ok && partial) {
+      const int i = 2 * n - 1, slot = i % kSlots;
+      if (mbar_wait_warp(&b_full[slot], (i / kSlots) & 1, kSitePrompt, lane)) {
+        const int valid = lk - (n - 1) * kKeys;
+        const uint32_t v = ring + slot * kTile;
+        for (int x = valid * 8 + lane; x < kKeys * 8; x += 32)
+          for (int h = 0; h < Cfg::kHalves; ++h)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * Cfg::kHalf + x * 16), "r"(0u) : "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(&b_fix);
+      }
+    }
+  } else if (w.q0 >= 0 && n > 0 && (warp == 9 || warp == 10)) {
+    // ---- MMA of tile i ----
+    if (lane == 0) {
+      const int i = warp - 9, mine = w.n[i];
+      const uint32_t id_s = pr_idesc(kKeys, false, p.negate != 0), id_o = pr_idesc(D, true, false);
+      const uint32_t ts = tmem + Cfg::kS + i * kKeys, tp = tmem + Cfg::kP + i * Cfg::kPCols, to = tmem + i * D;
+      auto full = [&](int x) { return mbar_wait(&b_full[x % kSlots], (x / kSlots) & 1, kSitePrompt); };
+      auto scores = [&](int j) {                         // S = Q K^T of tile j
+        const int x = 2 * j;
+        const uint32_t a = base + i * Cfg::kQTile, b = ring + (x % kSlots) * kTile;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ss(tmem + i * 128, pr_desc(a + (k >> 2) * 16384 + (k & 3) * 32, 16), pr_desc(b + (k >> 2) * 16384 + (k & 3) * 32, 16),
-                   id_s, k > 0);
-          mma_commit(&b_s[i]);
-        };
-        auto values = [&](int i, int at, bool first) {
-          const uint32_t b = ring + at * kTile;
-#pragma unroll
-          for (int k = 0; k < kPrKeys / 16; ++k)
-            mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, pr_desc(b + k * 2048, 16384), id_o, !first || k > 0);
-        };
-        ok = mbar_wait(&b_q, 0, kSitePrompt) && mbar_wait(&b_full[0], 0, kSitePrompt);
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(ts, pr_desc(a + (k >> 2) * 16384 + (k & 3) * 32, 16), pr_desc(b + (k >> 2) * Cfg::kHalf + (k & 3) * 32, 16),
+                 id_s, k > 0);
+        mma_commit(&b_s[i]);
+        mma_commit(&b_free[x % kSlots]);
+      };
+      if (mine > 0) {
+        ok = mbar_wait(&b_q, 0, kSitePrompt) && full(0);
         if (ok) {
           tc_fence_after();
-          scores(0, 0);
-          scores(1, 0);
-          mma_commit(&b_free[0]);
-          next();
+          scores(0);
         }
-        for (int j = 0; j < w.n && ok; ++j) {
-          const int v_slot = slot, v_round = round;
-          ok = mbar_wait(&b_full[v_slot], v_round & 1, kSitePrompt);
-          if (ok && j == w.n - 1 && partial) ok = mbar_wait(&b_fix, 0, kSitePrompt);
-          next();
-          const int k_slot = slot, k_round = round;
-          for (int i = 0; i < 2 && ok; ++i) {
-            ok = mbar_wait(&b_p[i], j & 1, kSitePrompt);
-            if (!ok) break;
-            tc_fence_after();
-            values(i, v_slot, j == 0);
-            if (j + 1 < w.n) {
-              if (i == 0) ok = mbar_wait(&b_full[k_slot], k_round & 1, kSitePrompt);
-              if (!ok) break;
-              scores(i, k_slot);
-            }
-          }
-          if (!ok) break;
-          mma_commit(&b_free[v_slot]);
-          if (j + 1 < w.n) {
-            mma_commit(&b_free[k_slot]);
-            next();
-          }
-        }
-        mma_commit(&b_o);
       }
-    } else if (warp < 8) {
-      // ---- softmax and output: one thread per row ----
-      const int i = warp >> 2, row = tid & 127;
-      const int tok = w.r0 + i * p.rows + row / p.group;        // token within the sequence
-      const int head = hk * p.group + row % p.group;
-      const bool live = row < p.rows * p.group && tok < lq;
-      int lim = lk;                                              // keys this row sees
-      if (p.causal) lim = max(0, min(lk, tok + 1 + lk - lq));
-      const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t ts = tmem + lane_base + i * 128, to = tmem + lane_base + 256 + i * 128;
-      const float c = p.scale_log2;
-      float m = -INFINITY, l = 0.0f;
-      for (int j = 0; j < w.n && ok; ++j) {
-        ok = mbar_wait_warp(&b_s[i], j & 1, kSitePrompt, lane);
+      for (int j = 0; j < mine && ok; ++j) {
+        if (j + 1 < mine) {
+          ok = full(2 * j + 2) && mbar_wait(&b_r[i], j & 1, kSitePrompt);
+          if (!ok) break;
+          tc_fence_after();
+          scores(j + 1);
+        }
+        const int x = 2 * j + 1;
+        ok = full(x) && (j < n - 1 || !partial || mbar_wait(&b_fix, 0, kSitePrompt)) && mbar_wait(&b_p[i], j & 1, kSitePrompt);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[128];
+        const uint32_t b = ring + (x % kSlots) * kTile;  // O += P V
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, s + 32 * x);
-        tmem_wait_ld();
-#pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_loaded32(s + 32 * x);
-        const int vis = lim - j * kPrKeys;
-        if (__any_sync(0xffffffffu, vis < kPrKeys)) {
-#pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x >= vis) s[x] = 0xff800000u;
-        }
-        float mx = __uint_as_float(s[0]);
-#pragma unroll
-        for (int x = 1; x < 128; ++x) mx = fmaxf(mx, __uint_as_float(s[x]));
-        // O keeps its reference maximum until a row's grows by more than 2^8
-        const bool move = (mx - m) * c > 8.0f || (m == -INFINITY && mx > -INFINITY);
-        if (__any_sync(0xffffffffu, move)) {
-          const float mn = fmaxf(m, mx);
-          if (j > 0) {
-            const float a = m == -INFINITY ? 0.0f : ex2f((m - mn) * c);
-            l *= a;
-            // (O of the tiles so far is complete: its products were issued before these scores)
-#pragma unroll 1
-            for (int x = 0; x < D; x += 32) {
-              uint32_t o[32];
-              tmem_ld32(to + x, o);
-              tmem_wait_ld();
-              tmem_loaded32(o);
-#pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
-              tmem_st32(to + x, o);
-            }
-          }
-          m = mn;
-        }
-        const float mc = m == -INFINITY ? 0.0f : m * c;
-        // weights in bf16 (half an ulp each, in [0, 2^8]); l sums the unrounded
-        float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 128; x += 32) {
-          uint32_t q[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            const float a = ex2f(__fmaf_rn(__uint_as_float(s[x + 2 * y]), c, -mc));
-            const float b = ex2f(__fmaf_rn(__uint_as_float(s[x + 2 * y + 1]), c, -mc));
-            sum0 += a;
-            sum1 += b;
-            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-            q[y] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          tmem_st16(ts + x / 2, q);
-        }
-        l += sum0 + sum1;
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&b_p[i]);
+        for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, tp + 8 * k, pr_desc(b + k * 2048, Cfg::kHalf), id_o, j > 0 || k > 0);
+        mma_commit(&b_o[i]);
+        mma_commit(&b_free[x % kSlots]);
       }
-      if (w.n > 0) ok = mbar_wait_warp(&b_o, 0, kSitePrompt, lane) && ok;
-      tc_fence_after();
-      const float r = l > 0.0f ? 1.0f / l : l;                   // a row that sees nothing: 0; NaN stays
-      __nv_bfloat16* dst = p.out + (static_cast<int64_t>(w.q0) + tok) * p.o_token + head * p.o_head;
-#pragma unroll 1
-      for (int x = 0; x < D; x += 32) {
-        uint32_t o[32];
-        if (w.n > 0) {
-          tmem_ld32(to + x, o);
-          tmem_wait_ld();
-          tmem_loaded32(o);
-        }
-        if (live) {
-#pragma unroll
-          for (int y = 0; y < 32; y += 8) {
-            float v[8];
-#pragma unroll
-            for (int z = 0; z < 8; ++z) v[z] = l == 0.0f ? 0.0f : __uint_as_float(o[y + z]) * r;
-            uint4 h;
-            uint32_t* hw = reinterpret_cast<uint32_t*>(&h);
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * z], v[2 * z + 1]);
-              hw[z] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            *reinterpret_cast<uint4*>(dst + x + y) = h;
-          }
-        }
+      // the tiles that only the other query tile sees
+      for (int x = 2 * mine; x < 2 * n && ok; ++x) {
+        ok = full(x);
+        if (ok) mbar_arrive(&b_free[x % kSlots]);
       }
-      if (live && p.lse)
-        p.lse[(static_cast<int64_t>(w.q0) + tok) * p.Hq + head] =
-            l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * c) + log2f(l)) * 0.6931471805599453f;
-      tc_fence_before();
+      if (!ok) mma_commit(&b_o[i]);                      // what has been issued
     }
+  } else if (w.q0 >= 0 && warp < 8) {
+    // ---- softmax and output: one thread per row ----
+    const int i = warp >> 2, row = tid & 127, mine = w.n[i];
+    const int tok = w.r0 + i * p.rows + row / p.group;        // token within the sequence
+    const int head = hk * p.group + row % p.group;
+    const bool live = row < p.rows * p.group && tok < lq;
+    int lim = lk;                                              // keys this row sees
+    if (p.causal) lim = max(0, min(lk, tok + 1 + lk - lq));
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t ts = lanes + Cfg::kS + i * kKeys, tp = lanes + Cfg::kP + i * Cfg::kPCols, to = lanes + i * D;
+    const float c = p.scale_log2;
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < mine && ok; ++j) {
+      ok = mbar_wait_warp(&b_s[i], j & 1, kSitePrompt, lane);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[kKeys];
+#pragma unroll
+      for (int x = 0; x < kKeys; x += 16) tmem_ld16r(ts + x, s + x);
+      tmem_wait_ld();
+#pragma unroll
+      for (int x = 0; x < kKeys; x += 16) tmem_loaded16(s + x);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b_r[i]);                     // the next scores may come
+      const int vis = lim - j * kKeys;
+      if (__any_sync(0xffffffffu, vis < kKeys)) {
+#pragma unroll
+        for (int x = 0; x < kKeys; ++x)
+          if (x >= vis) s[x] = 0xff800000u;
+      }
+      float mx8[8];
+#pragma unroll
+      for (int y = 0; y < 8; ++y) mx8[y] = fmaxf(__uint_as_float(s[y]), __uint_as_float(s[8 + y]));
+#pragma unroll
+      for (int x = 16; x < kKeys; x += 16)
+#pragma unroll
+        for (int y = 0; y < 8; ++y) mx8[y] = fmaxf(fmaxf(mx8[y], __uint_as_float(s[x + y])), __uint_as_float(s[x + 8 + y]));
+      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+      // O keeps its reference maximum until a row's grows by more than 2^60:
+      // fp32 and bf16 weights are as exact at any scale
+      const bool move = (mx - m) * c > 60.0f || (m == -INFINITY && mx > -INFINITY);
+      if (__any_sync(0xffffffffu, move)) {
+        const float mn = fmaxf(m, mx);
+        if (j > 0) {
+          // (the products of the tile before have updated O)
+          ok = mbar_wait_warp(&b_o[i], (j - 1) & 1, kSitePrompt, lane);
+          if (!ok) break;
+          tc_fence_after();
+          const float a = m == -INFINITY ? 0.0f : ex2f((m - mn) * c);
+          l *= a;
+#pragma unroll 1
+          for (int x = 0; x < D; x += 16) {
+            uint32_t o[16];
+            tmem_ld16r(to + x, o);
+            tmem_wait_ld();
+            tmem_loaded16(o);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
+            tmem_st16(to + x, o);
+          }
+        }
+        m = mn;
+      }
+      const float mc = m == -INFINITY ? 0.0f : m * c;
+      // weights in bf16 (half an ulp each); l sums the unrounded
+      const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
+      float2 sum[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) sum[y] = make_float2(0.0f, 0.0f);
+      uint32_t q[kKeys / 2];
+#pragma unroll
+      for (int y = 0; y < kKeys / 2; ++y) {
+        const float2 t = fma2(make_float2(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), c2, mc2);
+        const float2 e = make_float2(ex2f(t.x), ex2f(t.y));
+        sum[y & 3] = add2(sum[y & 3], e);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+        q[y] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      if (j > 0) {
+        // the products of the tile before have read P by now
+        ok = mbar_wait_warp(&b_o[i], (j - 1) & 1, kSitePrompt, lane);
+        if (!ok) break;
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int y = 0; y < kKeys / 2; y += 8) tmem_st8(tp + y, q + y);
+      const float2 sum2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+      l += sum2.x + sum2.y;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b_p[i]);
+    }
+    if (mine > 0) ok = mbar_wait_warp(&b_o[i], (mine - 1) & 1, kSitePrompt, lane) && ok;
+    else if (n > 0) ok = mbar_wait_warp(&b_q, 0, kSitePrompt, lane);      // q lands where the output is staged
+    tc_fence_after();
+    const float r = l > 0.0f ? 1.0f / l : l;                   // a row that sees nothing: 0; NaN stays
+    // through shared memory (this tile's q, which its last scores have read), so
+    // that a warp writes whole rows; chunks swizzled by row
+    const uint32_t stage = base + i * Cfg::kQTile;
+    constexpr int kChunks = D / 8;                             // 16-byte chunks of a row
+#pragma unroll 1
+    for (int x = 0; x < D; x += 16) {
+      uint32_t o[16];
+      if (mine > 0) {
+        tmem_ld16r(to + x, o);
+        tmem_wait_ld();
+        tmem_loaded16(o);
+      }
+#pragma unroll
+      for (int y = 0; y < 16; y += 8) {
+        uint32_t hw[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float v0 = l == 0.0f ? 0.0f : __uint_as_float(o[y + 2 * z]) * r;
+          const float v1 = l == 0.0f ? 0.0f : __uint_as_float(o[y + 2 * z + 1]) * r;
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v0, v1);
+          hw[z] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        const uint32_t at = stage + row * (2 * D) + (((x + y) / 8) ^ (row & 7)) * 16;
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hw[0]), "r"(hw[1]), "r"(hw[2]), "r"(hw[3]) : "memory");
+      }
+    }
+    __syncwarp();                                              // a warp stores the 32 rows that it wrote
+#pragma unroll 4
+    for (int x = lane; x < 32 * kChunks; x += 32) {
+      const int rr = (warp & 3) * 32 + x / kChunks, ch = x % kChunks;
+      const int tt = w.r0 + i * p.rows + rr / p.group;
+      if (rr < p.rows * p.group && tt < lq) {
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(stage + rr * (2 * D) + (ch ^ (rr & 7)) * 16) : "memory");
+        *reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(w.q0) + tt) * p.o_token +
+                                  (hk * p.group + rr % p.group) * p.o_head + 8 * ch) = v;
+      }
+    }
+    if (live && p.lse)
+      p.lse[(static_cast<int64_t>(w.q0) + tok) * p.Hq + head] =
+          l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * c) + log2f(l)) * 0.6931471805599453f;
+    tc_fence_before();
   }
   __syncthreads();
   if (warp == 9) {

@@ -297,10 +297,11 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
   p.scale_log2 = scale == 0.0f ? 1e-30f : std::fabs(scale) * 1.4426950408889634f;
   p.negate = scale < 0.0f;
   p.causal = causal ? 1 : 0;
+  const int keys = D == 128 ? PrCfg<128>::kKeys : PrCfg<64>::kKeys;
   CUtensorMap tq, tk, tv;
   if (!make_heads_tmap(&tq, q, Tq, Hq, D, q_token_stride, q_head_stride, group, p.rows) ||
-      !make_heads_tmap(&tk, Tk ? k : q, Tk ? Tk : 1, Hkv, D, Tk ? k_token_stride : 0, Tk ? k_head_stride : D, 1, kPrKeys) ||
-      !make_heads_tmap(&tv, Tk ? v : q, Tk ? Tk : 1, Hkv, D, Tk ? v_token_stride : 0, Tk ? v_head_stride : D, 1, kPrKeys))
+      !make_heads_tmap(&tk, Tk ? k : q, Tk ? Tk : 1, Hkv, D, Tk ? k_token_stride : 0, Tk ? k_head_stride : D, 1, keys) ||
+      !make_heads_tmap(&tv, Tk ? v : q, Tk ? Tk : 1, Hkv, D, Tk ? v_token_stride : 0, Tk ? v_head_stride : D, 1, keys))
     return FP8GQ_ERR_LAUNCH;
   // a row block more than the tokens fill for each sequence's odd end
   const int64_t blocks = (static_cast<int64_t>(Tq) / (2 * p.rows) + B) * Hkv;
