@@ -621,13 +621,17 @@ int fp8gq_paged_decode_attention(const void *q, int64_t q_token_stride, int64_t 
  * not written.  Values of other sequences never reach a row, NaN included; a
  * sequence's own k and v are taken to be finite (a masked v that is infinite
  * or NaN may reach the rows of its tile).  An offset out of range is cut to
- * [0, Tq] or [0, Tk] and recorded in the device error word. */
+ * [0, Tq] or [0, Tk] and recorded in the device error word.
+ * workspace: fp8gq_prompt_workspace_bytes bytes, as for fp8gq_paged_decode_attention.
+ * At most 128 query heads per kv head; scale is finite. */
+size_t fp8gq_prompt_workspace_bytes(void);
 int fp8gq_prompt_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
                            const void *k, int64_t k_token_stride, int64_t k_head_stride,
                            const void *v, int64_t v_token_stride, int64_t v_head_stride,
                            void *out, int64_t o_token_stride, int64_t o_head_stride, float *lse,
                            const int32_t *cu_q, const int32_t *cu_k, int B, int Tq, int Tk,
-                           int Hq, int Hkv, int D, float scale, int causal, fp8gq_stream_t stream);
+                           int Hq, int Hkv, int D, float scale, int causal,
+                           void *workspace, size_t workspace_bytes, fp8gq_stream_t stream);
 
 /* Log probabilities of given tokens under softmax(logits), with the entropy
  * and the `top_k` likeliest tokens of each row:

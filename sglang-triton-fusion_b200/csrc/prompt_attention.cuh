@@ -20,10 +20,17 @@
 // D = 128, the softmax waited 1900 of 4100 cycles a tile for the products and
 // 8192 tokens took 607 us.  v is read as it lies (its N side contiguous).
 //
+// One CTA per SM takes items (two query tiles of one kv head) off a common
+// counter, the last rows of a sequence first.  Every role runs on into the next
+// item as far as its barriers let it: the next q, k and v are on their way while
+// the last weights of this item are computed, its scores while its output is
+// written.  (A CTA per item spent 13000 cycles of its own before and after its
+// tiles: as much as 6 tiles take.)
+//
 // Warps 0-3 and 4-7: softmax, output (one thread per row of tile 0, 1).  Warp 8:
 // TMA; it also clears the rows of the last v tile that lie past the sequence
 // (another sequence's values, which a weight of 0 does not stop if they are
-// NaN).  Warps 9, 10: MMA of tile 0, 1.
+// NaN).  Warps 9, 10: MMA of tile 0, 1.  Warp 11: the items.
 #pragma once
 
 #include "fp8gq_device.cuh"
@@ -39,6 +46,8 @@ struct PromptParams {
   const int32_t* cu_k;
   int B, Tq, Tk, Hq, Hkv;
   int group, rows;          // query heads per kv head; tokens per query tile
+  int group_inv;            // 65536 / group, rounded up: x / group = x * group_inv >> 16 for x < 128
+  int* counters;            // [2], zero between launches: the next item, the CTAs that are done
   float scale_log2;         // |scale| log2(e)
   int negate;               // scale < 0
   int causal;
@@ -53,8 +62,9 @@ struct PrCfg {
   static constexpr int kQTile = kHalves * 128 * 128;       // bytes of a q tile
   static constexpr int kHalf = kKeys * 128;                // bytes of half a k or v tile (64 values)
   static constexpr int kTile = kHalves * kHalf;
-  static constexpr int kSlots = 8;                         // ring slots: k and v tiles in turn
-  static constexpr size_t kSmem = 1024 + 2 * static_cast<size_t>(kQTile) + kSlots * static_cast<size_t>(kTile);
+  static constexpr int kSlots = D == 128 ? 6 : 8;          // ring slots: k and v tiles in turn
+  static constexpr int kStage = 2 * 128 * 128;             // output on its way out: 64 values of each row
+  static constexpr size_t kSmem = 1024 + 2 * static_cast<size_t>(kQTile) + kStage + kSlots * static_cast<size_t>(kTile);
   // TMEM columns: O0 O1 S0 S1 P0 P1
   static constexpr int kS = 2 * D, kP = kS + 2 * kKeys, kPCols = (kKeys / 2 + 15) / 16 * 16;
   static_assert(kP + 2 * kPCols <= 512, "TMEM");
@@ -129,21 +139,14 @@ __device__ __forceinline__ float ex2f(float x) {
   return y;
 }
 
-// An offset cut to [0, hi]; one out of range is recorded.
-__device__ __forceinline__ int pr_cut(int x, int hi) {
-  if (x < 0 || x > hi) {
-    record_error(kSiteBadIndex);
-    return x < 0 ? 0 : hi;
-  }
-  return x;
-}
-
-// A CTA's work: two query tiles of one sequence and kv head.
+// An item: two query tiles of one sequence and kv head.
 struct PrWork {
-  int q0, q1, k0, k1;       // the sequence's tokens
-  int r0;                   // first token of the CTA within the sequence
+  int q0, lq, k0, lk;       // the sequence's tokens (q0 < 0: no more items)
+  int r0;                   // first token of the item within the sequence
+  int hk;
   int n[2];                 // key tiles that the last row of each query tile sees
 };
+constexpr int kPrItems = 2; // items looked up ahead
 
 template <int D>
 __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const __grid_constant__ CUtensorMap tq,
@@ -153,23 +156,32 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
   using Cfg = PrCfg<D>;
   constexpr int kSlots = Cfg::kSlots, kTile = Cfg::kTile, kKeys = Cfg::kKeys;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t b_q, b_fix;                        // q is there; the last v tile is cleared
+  __shared__ uint64_t b_item[kPrItems], b_taken[kPrItems];   // an item is there; every role has it behind it
+  __shared__ uint64_t b_want;                                // an item's loads are all on their way: time for the next
+  __shared__ uint64_t b_q, b_qfree, b_tail;                  // q is there; q is read; the last v tile is there
   __shared__ uint64_t b_full[kSlots], b_free[kSlots];
-  __shared__ uint64_t b_s[2], b_r[2], b_p[2], b_o[2];    // scores ready, read; weights ready; O updated
+  __shared__ uint64_t b_s[2], b_r[2], b_p[2], b_o[2];        // scores ready, read; weights ready; O updated
+  __shared__ uint64_t b_out[2];                              // O read
   __shared__ uint32_t s_tmem;
-  __shared__ int s_scan[kPrThreads / 32];
-  __shared__ PrWork s_work;
+  __shared__ PrWork s_work[kPrItems];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t ring = base + 2 * Cfg::kQTile;
+  const uint32_t out_stage = base + 2 * Cfg::kQTile;
+  const uint32_t ring = out_stage + Cfg::kStage;
 
   if (warp == 8) {
     if (lane == 0) {
       prefetch_tensormap(&tq);
       prefetch_tensormap(&tk);
       prefetch_tensormap(&tv);
+      for (int i = 0; i < kPrItems; ++i) {
+        mbar_init(&b_item[i], 1);
+        mbar_init(&b_taken[i], 11);       // TMA, 2 MMA, 8 softmax warps
+      }
+      mbar_init(&b_want, 1);
       mbar_init(&b_q, 1);
-      mbar_init(&b_fix, 32);
+      mbar_init(&b_qfree, 2);             // both MMA warps
+      mbar_init(&b_tail, 1);
       for (int i = 0; i < kSlots; ++i) {
         mbar_init(&b_full[i], 1);
         mbar_init(&b_free[i], 2);         // both MMA warps
@@ -179,6 +191,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         mbar_init(&b_r[i], 4);            // softmax warps
         mbar_init(&b_p[i], 4);
         mbar_init(&b_o[i], 1);
+        mbar_init(&b_out[i], 4);
       }
       fence_mbar_init();
     }
@@ -188,304 +201,393 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tc_fence_before();
   }
-  grid_dependency_wait();
-
-  // ---- the work of this CTA: row blocks of the sequences in order, the last
-  // (longest) of a sequence first ----
-  const int hk = blockIdx.x % p.Hkv, tile = blockIdx.x / p.Hkv;
-  const int span = 2 * p.rows;
-  const int share = (p.B + kPrThreads - 1) / kPrThreads;
-  const int b_lo = min(tid * share, p.B), b_hi = min(b_lo + share, p.B);
-  auto tokens = [&](int b, int& q0, int& q1) {
-    q0 = pr_cut(__ldg(p.cu_q + b), p.Tq);
-    q1 = pr_cut(__ldg(p.cu_q + b + 1), p.Tq);
-    if (q1 < q0) {
-      record_error(kSiteBadIndex);
-      q1 = q0;
-    }
-  };
-  int mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) {
-    int q0, q1;
-    tokens(b, q0, q1);
-    mine += (q1 - q0 + span - 1) / span;
-  }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
-  }
-  if (lane == 31) s_scan[warp] = incl;
-  if (tid == 0) s_work.q0 = -1;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) incl += s_scan[w];
-  if (tile < incl && tile >= incl - mine) {
-    int at = incl - mine;
-    for (int b = b_lo; b < b_hi; ++b) {
-      PrWork w;
-      tokens(b, w.q0, w.q1);
-      const int nb = (w.q1 - w.q0 + span - 1) / span;
-      if (tile < at + nb) {
-        w.k0 = pr_cut(__ldg(p.cu_k + b), p.Tk);
-        w.k1 = pr_cut(__ldg(p.cu_k + b + 1), p.Tk);
-        if (w.k1 < w.k0) {
-          record_error(kSiteBadIndex);
-          w.k1 = w.k0;
-        }
-        w.r0 = (nb - 1 - (tile - at)) * span;
-        const int lq = w.q1 - w.q0, lk = w.k1 - w.k0;
-        for (int i = 0; i < 2; ++i) {
-          const int end = min(w.r0 + (i + 1) * p.rows, lq);       // past the tile's last token
-          int seen = end > w.r0 + i * p.rows ? lk : 0;
-          if (p.causal && seen) seen = min(lk, max(0, end + lk - lq));
-          w.n[i] = (seen + kKeys - 1) / kKeys;
-        }
-        s_work = w;
-        break;
-      }
-      at += nb;
-    }
-  }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const PrWork w = s_work;
-  const int lq = w.q1 - w.q0, lk = w.k1 - w.k0;
-  const int n = max(w.n[0], w.n[1]);
-  const bool partial = n * kKeys > lk;           // the last tile reaches past the sequence
+  grid_dependency_wait();
   bool ok = true;
 
-  if (w.q0 >= 0 && n > 0 && warp == 8) {
-    // ---- TMA ----
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
-      for (int i = 0; i < 2; ++i)
-        for (int h = 0; h < Cfg::kHalves; ++h)
-          tma_load_3d(base + i * Cfg::kQTile + h * 16384, &tq, 64 * h, hk * p.group, w.q0 + w.r0 + i * p.rows, &b_q);
-      int slot = 0, round = 0, issued = 0;
-      for (int i = 0; i < 2 * n && ok; ++i) {            // k and v tiles in turn
-        if (round > 0) ok = mbar_wait(&b_free[slot], (round - 1) & 1, kSitePrompt);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&b_full[slot], kTile);
-        for (int h = 0; h < Cfg::kHalves; ++h)
-          tma_load_3d(ring + slot * kTile + h * Cfg::kHalf, (i & 1) ? &tv : &tk, 64 * h, hk, w.k0 + (i >> 1) * kKeys,
-                      &b_full[slot]);
-        ++issued;
-        if (++slot == kSlots) {
-          slot = 0;
-          ++round;
+  // The items as every role sees them; k and v tiles and steps are numbered
+  // through all items.
+  int item = 0;
+  PrWork w;
+  auto next_item = [&]() {
+    ok = mbar_wait_warp(&b_item[item % kPrItems], (item / kPrItems) & 1, kSitePrompt, lane) && ok;
+    if (!ok) return false;
+    w = s_work[item % kPrItems];
+    return w.q0 >= 0;
+  };
+  auto leave_item = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&b_taken[item % kPrItems]);
+    ++item;
+  };
+
+  if (warp >= 8) {
+    if (warp == 11) {
+      // ---- items ----
+      const int span = 2 * p.rows;
+      const int share = (p.B + 31) / 32;
+      const int b_lo = min(lane * share, p.B), b_hi = min(b_lo + share, p.B);
+      auto tokens = [&](int b, int& q0, int& q1, bool record) {
+        q0 = __ldg(p.cu_q + b);
+        q1 = __ldg(p.cu_q + b + 1);
+        if (q0 < 0 || q0 > p.Tq || q1 < q0 || q1 > p.Tq) {
+          if (record) record_error(kSiteBadIndex);
+          q0 = min(max(q0, 0), p.Tq);
+          q1 = min(max(q1, q0), p.Tq);
         }
-      }
-      if (!ok) {
-        // gave up: let the copies in flight land before the CTA may end
-        mbar_wait(&b_q, 0, kSitePrompt);
-        for (int i = issued > kSlots ? issued - kSlots : 0; i < issued; ++i)
-          mbar_wait(&b_full[i % kSlots], (i / kSlots) & 1, kSitePrompt);
-      }
-    }
-    // the last v tile's rows past the sequence: zeros
-    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-    if (ok && partial) {
-      const int i = 2 * n - 1, slot = i % kSlots;
-      if (mbar_wait_warp(&b_full[slot], (i / kSlots) & 1, kSitePrompt, lane)) {
-        const int valid = lk - (n - 1) * kKeys;
-        const uint32_t v = ring + slot * kTile;
-        for (int x = valid * 8 + lane; x < kKeys * 8; x += 32)
-          for (int h = 0; h < Cfg::kHalves; ++h)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * Cfg::kHalf + x * 16), "r"(0u) : "memory");
-        fence_proxy_async_smem();
-        mbar_arrive(&b_fix);
-      }
-    }
-  } else if (w.q0 >= 0 && n > 0 && (warp == 9 || warp == 10)) {
-    // ---- MMA of tile i ----
-    if (lane == 0) {
-      const int i = warp - 9, mine = w.n[i];
-      const uint32_t id_s = pr_idesc(kKeys, false, p.negate != 0), id_o = pr_idesc(D, true, false);
-      const uint32_t ts = tmem + Cfg::kS + i * kKeys, tp = tmem + Cfg::kP + i * Cfg::kPCols, to = tmem + i * D;
-      auto full = [&](int x) { return mbar_wait(&b_full[x % kSlots], (x / kSlots) & 1, kSitePrompt); };
-      auto scores = [&](int j) {                         // S = Q K^T of tile j
-        const int x = 2 * j;
-        const uint32_t a = base + i * Cfg::kQTile, b = ring + (x % kSlots) * kTile;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_ss(ts, pr_desc(a + (k >> 2) * 16384 + (k & 3) * 32, 16), pr_desc(b + (k >> 2) * Cfg::kHalf + (k & 3) * 32, 16),
-                 id_s, k > 0);
-        mma_commit(&b_s[i]);
-        mma_commit(&b_free[x % kSlots]);
       };
-      if (mine > 0) {
-        ok = mbar_wait(&b_q, 0, kSitePrompt) && full(0);
-        if (ok) {
-          tc_fence_after();
-          scores(0);
-        }
+      int mine = 0;
+      for (int b = b_lo; b < b_hi; ++b) {
+        int q0, q1;
+        tokens(b, q0, q1, blockIdx.x == 0);
+        mine += (q1 - q0 + span - 1) / span;
       }
-      for (int j = 0; j < mine && ok; ++j) {
-        if (j + 1 < mine) {
-          ok = full(2 * j + 2) && mbar_wait(&b_r[i], j & 1, kSitePrompt);
-          if (!ok) break;
-          tc_fence_after();
-          scores(j + 1);
-        }
-        const int x = 2 * j + 1;
-        ok = full(x) && (j < n - 1 || !partial || mbar_wait(&b_fix, 0, kSitePrompt)) && mbar_wait(&b_p[i], j & 1, kSitePrompt);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t b = ring + (x % kSlots) * kTile;  // O += P V
+      int incl = mine;
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, tp + 8 * k, pr_desc(b + k * 2048, Cfg::kHalf), id_o, j > 0 || k > 0);
-        mma_commit(&b_o[i]);
-        mma_commit(&b_free[x % kSlots]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
       }
-      // the tiles that only the other query tile sees
-      for (int x = 2 * mine; x < 2 * n && ok; ++x) {
-        ok = full(x);
-        if (ok) mbar_arrive(&b_free[x % kSlots]);
-      }
-      if (!ok) mma_commit(&b_o[i]);                      // what has been issued
-    }
-  } else if (w.q0 >= 0 && warp < 8) {
-    // ---- softmax and output: one thread per row ----
-    const int i = warp >> 2, row = tid & 127, mine = w.n[i];
-    const int tok = w.r0 + i * p.rows + row / p.group;        // token within the sequence
-    const int head = hk * p.group + row % p.group;
-    const bool live = row < p.rows * p.group && tok < lq;
-    int lim = lk;                                              // keys this row sees
-    if (p.causal) lim = max(0, min(lk, tok + 1 + lk - lq));
-    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t ts = lanes + Cfg::kS + i * kKeys, tp = lanes + Cfg::kP + i * Cfg::kPCols, to = lanes + i * D;
-    const float c = p.scale_log2;
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < mine && ok; ++j) {
-      ok = mbar_wait_warp(&b_s[i], j & 1, kSitePrompt, lane);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[kKeys];
-#pragma unroll
-      for (int x = 0; x < kKeys; x += 16) tmem_ld16r(ts + x, s + x);
-      tmem_wait_ld();
-#pragma unroll
-      for (int x = 0; x < kKeys; x += 16) tmem_loaded16(s + x);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b_r[i]);                     // the next scores may come
-      const int vis = lim - j * kKeys;
-      if (__any_sync(0xffffffffu, vis < kKeys)) {
-#pragma unroll
-        for (int x = 0; x < kKeys; ++x)
-          if (x >= vis) s[x] = 0xff800000u;
-      }
-      float mx8[8];
-#pragma unroll
-      for (int y = 0; y < 8; ++y) mx8[y] = fmaxf(__uint_as_float(s[y]), __uint_as_float(s[8 + y]));
-#pragma unroll
-      for (int x = 16; x < kKeys; x += 16)
-#pragma unroll
-        for (int y = 0; y < 8; ++y) mx8[y] = fmaxf(fmaxf(mx8[y], __uint_as_float(s[x + y])), __uint_as_float(s[x + 8 + y]));
-      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-      // O keeps its reference maximum until a row's grows by more than 2^60:
-      // fp32 and bf16 weights are as exact at any scale
-      const bool move = (mx - m) * c > 60.0f || (m == -INFINITY && mx > -INFINITY);
-      if (__any_sync(0xffffffffu, move)) {
-        const float mn = fmaxf(m, mx);
-        if (j > 0) {
-          // (the products of the tile before have updated O)
-          ok = mbar_wait_warp(&b_o[i], (j - 1) & 1, kSitePrompt, lane);
-          if (!ok) break;
-          tc_fence_after();
-          const float a = m == -INFINITY ? 0.0f : ex2f((m - mn) * c);
-          l *= a;
-#pragma unroll 1
-          for (int x = 0; x < D; x += 16) {
-            uint32_t o[16];
-            tmem_ld16r(to + x, o);
-            tmem_wait_ld();
-            tmem_loaded16(o);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
-            tmem_st16(to + x, o);
+      const int total = __shfl_sync(0xffffffffu, incl, 31) * p.Hkv;
+      int id = blockIdx.x;                          // the first item; the others off the counter
+      for (int it = 0;; ++it) {
+        PrWork x;
+        x.q0 = -1;
+        const int tile = id / p.Hkv;
+        const bool here = id < total && tile < incl && tile >= incl - mine;
+        if (here) {
+          int at = incl - mine;
+          for (int b = b_lo; b < b_hi; ++b) {
+            int q0, q1;
+            tokens(b, q0, q1, false);
+            const int nb = (q1 - q0 + span - 1) / span;
+            if (tile < at + nb) {
+              int k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
+              if (k0 < 0 || k0 > p.Tk || k1 < k0 || k1 > p.Tk) {
+                record_error(kSiteBadIndex);
+                k0 = min(max(k0, 0), p.Tk);
+                k1 = min(max(k1, k0), p.Tk);
+              }
+              x.q0 = q0;
+              x.lq = q1 - q0;
+              x.k0 = k0;
+              x.lk = k1 - k0;
+              x.hk = id - tile * p.Hkv;
+              x.r0 = (nb - 1 - (tile - at)) * span;
+              for (int i = 0; i < 2; ++i) {
+                const int end = min(x.r0 + (i + 1) * p.rows, x.lq);      // past the query tile's last token
+                int seen = end > x.r0 + i * p.rows ? x.lk : 0;
+                if (p.causal && seen) seen = min(x.lk, max(0, end + x.lk - x.lq));
+                x.n[i] = (seen + kKeys - 1) / kKeys;
+              }
+              break;
+            }
+            at += nb;
           }
         }
-        m = mn;
+        if (it >= kPrItems) ok = mbar_wait_warp(&b_taken[it % kPrItems], (it / kPrItems - 1) & 1, kSitePrompt, lane);
+        if (!ok) break;
+        if (here || (lane == 0 && id >= total)) s_work[it % kPrItems] = x;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_item[it % kPrItems]);
+        if (id >= total) break;
+        // not before this item's loads are issued: an item taken early is one that
+        // an idle CTA cannot take
+        ok = mbar_wait_warp(&b_want, it & 1, kSitePrompt, lane);
+        if (!ok) break;
+        if (lane == 0) id = gridDim.x + atomicAdd(p.counters, 1);
+        id = __shfl_sync(0xffffffffu, id, 0);
       }
-      const float mc = m == -INFINITY ? 0.0f : m * c;
-      // weights in bf16 (half an ulp each); l sums the unrounded
-      const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
-      float2 sum[4];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) sum[y] = make_float2(0.0f, 0.0f);
-      uint32_t q[kKeys / 2];
-#pragma unroll
-      for (int y = 0; y < kKeys / 2; ++y) {
-        const float2 t = fma2(make_float2(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), c2, mc2);
-        const float2 e = make_float2(ex2f(t.x), ex2f(t.y));
-        sum[y & 3] = add2(sum[y & 3], e);
-        const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
-        q[y] = *reinterpret_cast<const uint32_t*>(&h);
+      // the last CTA to get here leaves the counters as it found them
+      if (lane == 0) {
+        __threadfence();
+        if (atomicAdd(p.counters + 1, 1) == static_cast<int>(gridDim.x) - 1) {
+          p.counters[0] = 0;
+          p.counters[1] = 0;
+        }
       }
-      if (j > 0) {
-        // the products of the tile before have read P by now
-        ok = mbar_wait_warp(&b_o[i], (j - 1) & 1, kSitePrompt, lane);
+    } else if (warp == 8) {
+      // ---- TMA ----
+      int x0 = 0, items = 0, tails = 0;             // k and v tiles, items and tails so far
+      while (next_item()) {
+        const int n = max(w.n[0], w.n[1]);
+        const bool partial = n * kKeys > w.lk;      // the last tile reaches past the sequence
+        if (n > 0) {
+          if (lane == 0) {
+            if (items > 0) ok = mbar_wait(&b_qfree, (items - 1) & 1, kSitePrompt);
+            if (ok) {
+              mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
+              for (int i = 0; i < 2; ++i)
+                for (int h = 0; h < Cfg::kHalves; ++h)
+                  tma_load_3d(base + i * Cfg::kQTile + h * 16384, &tq, 64 * h, w.hk * p.group, w.q0 + w.r0 + i * p.rows, &b_q);
+            }
+            for (int i = 0; i < 2 * n && ok; ++i) {            // k and v tiles in turn
+              const int x = x0 + i, slot = x % kSlots;
+              if (x >= kSlots) ok = mbar_wait(&b_free[slot], (x / kSlots - 1) & 1, kSitePrompt);
+              if (!ok) break;
+              uint64_t* bar = partial && i == 2 * n - 1 ? &b_tail : &b_full[slot];
+              mbar_arrive_expect_tx(bar, kTile);
+              for (int h = 0; h < Cfg::kHalves; ++h)
+                tma_load_3d(ring + slot * kTile + h * Cfg::kHalf, (i & 1) ? &tv : &tk, 64 * h, w.hk, w.k0 + (i >> 1) * kKeys, bar);
+            }
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (!ok) break;
+          if (partial) {
+            // rows past the sequence: zeros, then the tile is there
+            const int slot = (x0 + 2 * n - 1) % kSlots, valid = w.lk - (n - 1) * kKeys;
+            ok = mbar_wait_warp(&b_tail, tails & 1, kSitePrompt, lane);
+            if (!ok) break;
+            for (int x = valid * 8 + lane; x < kKeys * 8; x += 32)
+              for (int h = 0; h < Cfg::kHalves; ++h)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + slot * kTile + h * Cfg::kHalf + x * 16), "r"(0u)
+                             : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b_full[slot]);
+            ++tails;
+          }
+          x0 += 2 * n;
+          ++items;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_want);
+        leave_item();
+      }
+      // the copies that no one has waited for have landed before the CTA ends
+      // (only after a wait gave up: otherwise every tile has been used)
+      if (!ok && lane == 0) {
+        mbar_wait(&b_q, items & 1, kSitePrompt);
+        for (int i = 0; i < kSlots; ++i) mbar_wait(&b_full[i], (x0 / kSlots) & 1, kSitePrompt);
+      }
+    } else {
+      // ---- MMA of tile i ----
+      const int i = warp - 9;
+      const uint32_t id_s = pr_idesc(kKeys, false, p.negate != 0), id_o = pr_idesc(D, true, false);
+      const uint32_t ts = tmem + Cfg::kS + i * kKeys, tp = tmem + Cfg::kP + i * Cfg::kPCols, to = tmem + i * D;
+      int x0 = 0, items = 0, step0 = 0, outs = 0;   // tiles, items with tiles, this tile's steps and outputs so far
+      while (next_item()) {
+        const int mine = w.n[i], n = max(w.n[0], w.n[1]);
+        if (n > 0 && lane == 0) {
+          auto full = [&](int x) { return mbar_wait(&b_full[x % kSlots], (x / kSlots) & 1, kSitePrompt); };
+          auto scores = [&](int j) {                       // S = Q K^T of tile j
+            const int x = x0 + 2 * j, step = step0 + j;
+            ok = full(x) && (step == 0 || mbar_wait(&b_r[i], (step - 1) & 1, kSitePrompt));
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t a = base + i * Cfg::kQTile, b = ring + (x % kSlots) * kTile;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              mma_ss(ts, pr_desc(a + (k >> 2) * 16384 + (k & 3) * 32, 16), pr_desc(b + (k >> 2) * Cfg::kHalf + (k & 3) * 32, 16),
+                     id_s, k > 0);
+            mma_commit(&b_s[i]);
+            mma_commit(&b_free[x % kSlots]);
+          };
+          ok = mbar_wait(&b_q, items & 1, kSitePrompt);
+          if (ok && mine > 0) scores(0);
+          for (int j = 0; j < mine && ok; ++j) {
+            if (j + 1 < mine) {
+              scores(j + 1);
+              if (!ok) break;
+            }
+            if (j + 1 >= mine) mma_commit(&b_qfree);                     // q has been read
+            const int x = x0 + 2 * j + 1;
+            ok = full(x) && mbar_wait(&b_p[i], (step0 + j) & 1, kSitePrompt) &&
+                 (j > 0 || outs == 0 || mbar_wait(&b_out[i], (outs - 1) & 1, kSitePrompt));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t b = ring + (x % kSlots) * kTile;              // O += P V
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, tp + 8 * k, pr_desc(b + k * 2048, Cfg::kHalf), id_o, j > 0 || k > 0);
+            mma_commit(&b_free[x % kSlots]);
+            mma_commit(&b_o[i]);                                         // (the last commit of an item)
+          }
+          if (mine == 0) mbar_arrive(&b_qfree);
+          // the tiles that only the other query tile sees
+          for (int x = 2 * mine; x < 2 * n && ok; ++x) {
+            ok = full(x0 + x);
+            if (ok) mbar_arrive(&b_free[(x0 + x) % kSlots]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        if (n > 0) ++items;
+        x0 += 2 * n;
+        step0 += mine;
+        if (mine > 0) ++outs;
+        leave_item();
+      }
+      if (!ok && lane == 0) {                              // what has been issued completes
+        mma_commit(&b_o[i]);
+        mbar_wait(&b_o[i], step0 & 1, kSitePrompt);
+      }
+    }
+  } else {
+    // ---- softmax and output: one thread per row ----
+    const int i = warp >> 2, row = tid & 127;
+    const int row_tok = (row * p.group_inv) >> 16, row_head = row - row_tok * p.group;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t ts = lanes + Cfg::kS + i * kKeys, tp = lanes + Cfg::kP + i * Cfg::kPCols, to = lanes + i * D;
+    const uint32_t stage = out_stage + warp * 4096;        // 32 rows of 64 values
+    const float c = p.scale_log2;
+    int step0 = 0;                                         // this tile's steps so far
+    while (next_item()) {
+      const int mine = w.n[i];
+      const int tok = w.r0 + i * p.rows + row_tok;         // token within the sequence
+      const bool live = row_tok < p.rows && tok < w.lq;
+      int lim = w.lk;                                      // keys this row sees
+      if (p.causal) lim = max(0, min(w.lk, tok + 1 + w.lk - w.lq));
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < mine; ++j) {
+        const int step = step0 + j;
+        ok = mbar_wait_warp(&b_s[i], step & 1, kSitePrompt, lane);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[kKeys];
+#pragma unroll
+        for (int x = 0; x < kKeys; x += 16) tmem_ld16r(ts + x, s + x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < kKeys; x += 16) tmem_loaded16(s + x);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_r[i]);               // the next scores may come
+        const int vis = lim - j * kKeys;
+        if (__any_sync(0xffffffffu, vis < kKeys)) {
+#pragma unroll
+          for (int x = 0; x < kKeys; ++x)
+            if (x >= vis) s[x] = 0xff800000u;
+        }
+        float mx8[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) mx8[y] = fmaxf(__uint_as_float(s[y]), __uint_as_float(s[8 + y]));
+#pragma unroll
+        for (int x = 16; x < kKeys; x += 16)
+#pragma unroll
+          for (int y = 0; y < 8; ++y) mx8[y] = fmaxf(fmaxf(mx8[y], __uint_as_float(s[x + y])), __uint_as_float(s[x + 8 + y]));
+        const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+        // O keeps its reference maximum until a row's grows by more than 2^60:
+        // fp32 and bf16 weights are as exact at any scale
+        const bool move = (mx - m) * c > 60.0f || (m == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, move)) {
+          const float mn = fmaxf(m, mx);
+          if (j > 0) {
+            // (the products of the tile before have updated O)
+            ok = mbar_wait_warp(&b_o[i], (step - 1) & 1, kSitePrompt, lane);
+            if (!ok) break;
+            tc_fence_after();
+            const float a = m == -INFINITY ? 0.0f : ex2f((m - mn) * c);
+            l *= a;
+#pragma unroll 1
+            for (int x = 0; x < D; x += 16) {
+              uint32_t o[16];
+              tmem_ld16r(to + x, o);
+              tmem_wait_ld();
+              tmem_loaded16(o);
+#pragma unroll
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * a);
+              tmem_st16(to + x, o);
+            }
+          }
+          m = mn;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        // weights in bf16 (half an ulp each); l sums the unrounded
+        const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
+        float2 sum[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) sum[y] = make_float2(0.0f, 0.0f);
+        constexpr int kPart = kKeys > 80 ? kKeys / 2 : kKeys;          // (registers)
+#pragma unroll
+        for (int x = 0; x < kKeys; x += kPart) {
+          uint32_t q[kPart / 2];
+#pragma unroll
+          for (int y = 0; y < kPart / 2; ++y) {
+            const float2 t = fma2(make_float2(__uint_as_float(s[x + 2 * y]), __uint_as_float(s[x + 2 * y + 1])), c2, mc2);
+            const float2 e = make_float2(ex2f(t.x), ex2f(t.y));
+            sum[y & 3] = add2(sum[y & 3], e);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+            q[y] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          if (x == 0 && step > 0) {
+            // the products of the tile before have read P by now
+            ok = mbar_wait_warp(&b_o[i], (step - 1) & 1, kSitePrompt, lane);
+            if (!ok) break;
+            tc_fence_after();
+          }
+#pragma unroll
+          for (int y = 0; y < kPart / 2; y += 8) tmem_st8(tp + x / 2 + y, q + y);
+        }
+        if (!ok) break;
+        const float2 sum2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += sum2.x + sum2.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_p[i]);
+      }
+      if (!ok) break;
+      step0 += mine;
+      if (mine > 0) {
+        ok = mbar_wait_warp(&b_o[i], (step0 - 1) & 1, kSitePrompt, lane);
         if (!ok) break;
         tc_fence_after();
       }
-#pragma unroll
-      for (int y = 0; y < kKeys / 2; y += 8) tmem_st8(tp + y, q + y);
-      const float2 sum2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-      l += sum2.x + sum2.y;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b_p[i]);
-    }
-    if (mine > 0) ok = mbar_wait_warp(&b_o[i], (mine - 1) & 1, kSitePrompt, lane) && ok;
-    else if (n > 0) ok = mbar_wait_warp(&b_q, 0, kSitePrompt, lane);      // q lands where the output is staged
-    tc_fence_after();
-    const float r = l > 0.0f ? 1.0f / l : l;                   // a row that sees nothing: 0; NaN stays
-    // through shared memory (this tile's q, which its last scores have read), so
-    // that a warp writes whole rows; chunks swizzled by row
-    const uint32_t stage = base + i * Cfg::kQTile;
-    constexpr int kChunks = D / 8;                             // 16-byte chunks of a row
+      const float r = l > 0.0f ? 1.0f / l : l;             // a row that sees nothing: 0; NaN stays
+      // 64 values of each row at a time through shared memory (chunks swizzled
+      // by row), so that the warp writes whole rows
 #pragma unroll 1
-    for (int x = 0; x < D; x += 16) {
-      uint32_t o[16];
-      if (mine > 0) {
-        tmem_ld16r(to + x, o);
-        tmem_wait_ld();
-        tmem_loaded16(o);
-      }
+      for (int half = 0; half < Cfg::kHalves; ++half) {
+        __syncwarp();                                      // the half before is on its way
 #pragma unroll
-      for (int y = 0; y < 16; y += 8) {
-        uint32_t hw[4];
+        for (int q = 0; q < 64; q += 16) {
+          uint32_t o[16];
+          if (mine > 0) {
+            tmem_ld16r(to + 64 * half + q, o);
+            tmem_wait_ld();
+            tmem_loaded16(o);
+          }
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const float v0 = l == 0.0f ? 0.0f : __uint_as_float(o[y + 2 * z]) * r;
-          const float v1 = l == 0.0f ? 0.0f : __uint_as_float(o[y + 2 * z + 1]) * r;
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v0, v1);
-          hw[z] = *reinterpret_cast<const uint32_t*>(&b);
+          for (int x = 0; x < 2; ++x) {
+            uint32_t hw[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const float v0 = l == 0.0f ? 0.0f : __uint_as_float(o[8 * x + 2 * z]) * r;
+              const float v1 = l == 0.0f ? 0.0f : __uint_as_float(o[8 * x + 2 * z + 1]) * r;
+              const __nv_bfloat162 b = __floats2bfloat162_rn(v0, v1);
+              hw[z] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((q / 8 + x) ^ (lane & 7)) * 16),
+                         "r"(hw[0]), "r"(hw[1]), "r"(hw[2]), "r"(hw[3]) : "memory");
+          }
         }
-        const uint32_t at = stage + row * (2 * D) + (((x + y) / 8) ^ (row & 7)) * 16;
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hw[0]), "r"(hw[1]), "r"(hw[2]), "r"(hw[3]) : "memory");
+        if (half == Cfg::kHalves - 1 && mine > 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b_out[i]);           // O may be overwritten
+        }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int rr = 4 * x + (lane >> 3), ch = lane & 7;           // row within the warp, chunk
+          const int rt = (((warp & 3) * 32 + rr) * p.group_inv) >> 16, rh = (warp & 3) * 32 + rr - rt * p.group;
+          const int tt = w.r0 + i * p.rows + rt;
+          if (rt < p.rows && tt < w.lq) {
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(stage + rr * 128 + (ch ^ (rr & 7)) * 16) : "memory");
+            *reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(w.q0) + tt) * p.o_token +
+                                      (w.hk * p.group + rh) * p.o_head + 64 * half + 8 * ch) = v;
+          }
+        }
       }
+      if (live && p.lse)
+        p.lse[(static_cast<int64_t>(w.q0) + tok) * p.Hq + w.hk * p.group + row_head] =
+            l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * c) + log2f(l)) * 0.6931471805599453f;
+      leave_item();
     }
-    __syncwarp();                                              // a warp stores the 32 rows that it wrote
-#pragma unroll 4
-    for (int x = lane; x < 32 * kChunks; x += 32) {
-      const int rr = (warp & 3) * 32 + x / kChunks, ch = x % kChunks;
-      const int tt = w.r0 + i * p.rows + rr / p.group;
-      if (rr < p.rows * p.group && tt < lq) {
-        uint4 v;
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                     : "r"(stage + rr * (2 * D) + (ch ^ (rr & 7)) * 16) : "memory");
-        *reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(w.q0) + tt) * p.o_token +
-                                  (hk * p.group + rr % p.group) * p.o_head + 8 * ch) = v;
-      }
-    }
-    if (live && p.lse)
-      p.lse[(static_cast<int64_t>(w.q0) + tok) * p.Hq + head] =
-          l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * c) + log2f(l)) * 0.6931471805599453f;
     tc_fence_before();
   }
   __syncthreads();

@@ -80,6 +80,8 @@ int check_rows(const void* p, int64_t token, int64_t head, int tokens, int heads
 }
 
 // ----------------------------------------------------------------- prompt --
+constexpr size_t kPromptWorkspaceBytes = 16;
+
 // [tokens, heads, D] bf16 as boxes of 64 values x `box_heads` heads x
 // `box_tokens` tokens, 128-byte swizzle.  A stride that no coordinate above 0
 // uses is replaced by a valid one.
@@ -258,11 +260,13 @@ int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t 
   return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_paged_decode_attention");
 }
 
+size_t fp8gq_prompt_workspace_bytes(void) { return kPromptWorkspaceBytes; }
+
 int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                            int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                            int64_t v_head_stride, void* out, int64_t o_token_stride, int64_t o_head_stride, float* lse,
                            const int32_t* cu_q, const int32_t* cu_k, int B, int Tq, int Tk, int Hq, int Hkv, int D,
-                           float scale, int causal, fp8gq_stream_t stream) {
+                           float scale, int causal, void* workspace, size_t workspace_bytes, fp8gq_stream_t stream) {
   if (B < 0 || Tq < 0 || Tk < 0) return FP8GQ_ERR_SHAPE;
   int st = check_heads(Hq, Hkv, D);
   if (st != FP8GQ_OK) return st;
@@ -293,6 +297,7 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
   p.Hkv = Hkv;
   p.group = group;
   p.rows = 128 / group;
+  p.group_inv = (65536 + group - 1) / group;
   // a scale of 0 as one too small to tell scores apart, so that -inf stays -inf
   p.scale_log2 = scale == 0.0f ? 1e-30f : std::fabs(scale) * 1.4426950408889634f;
   p.negate = scale < 0.0f;
@@ -304,8 +309,12 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
       !make_heads_tmap(&tv, Tk ? v : q, Tk ? Tk : 1, Hkv, D, Tk ? v_token_stride : 0, Tk ? v_head_stride : D, 1, keys))
     return FP8GQ_ERR_LAUNCH;
   // a row block more than the tokens fill for each sequence's odd end
-  const int64_t blocks = (static_cast<int64_t>(Tq) / (2 * p.rows) + B) * Hkv;
-  if (blocks > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
+  int64_t blocks = (static_cast<int64_t>(Tq) / (2 * p.rows) + B) * Hkv;
+  if (blocks > INT32_MAX / 2) return FP8GQ_ERR_UNSUPPORTED;
+  if (blocks > di.sm_count) blocks = di.sm_count;
+  if (!workspace || workspace_bytes < kPromptWorkspaceBytes) return FP8GQ_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return FP8GQ_ERR_ALIGNMENT;
+  p.counters = static_cast<int*>(workspace);
   auto fn = D == 128 ? prompt_attention_kernel<128> : prompt_attention_kernel<64>;
   const size_t smem = D == 128 ? PrCfg<128>::kSmem : PrCfg<64>::kSmem;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(fn), static_cast<int>(smem));

@@ -24,6 +24,7 @@ from .ops import RMS_EPS, ShapeError, _check_cuda, _stream, _workspace_entry
 
 HEAD_DIMS = (64, 128)
 MAX_TOP = 32
+PROMPT_WORKSPACE = 16   # fp8gq_prompt_workspace_bytes()
 _BF16, _E4M3, _F32 = 0, 1, 2   # FP8GQ_DTYPE_*
 _byref = ctypes.byref
 _decode_ws_bytes: dict = {}    # (device, Hq, Hkv, D) -> fp8gq_paged_decode_workspace_bytes
@@ -188,10 +189,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if shape != q.shape:
             raise ShapeError(f"out must be {tuple(q.shape)}, got {tuple(shape)}")
     lse = torch.empty((tq, hq), dtype=torch.float32, device=dev) if return_lse else None
+    stream = _stream(dev)
+    _, ws_ptr, ws_n = _workspace_entry(dev, PROMPT_WORKSPACE, stream)
     st = _lib.load().fp8gq_prompt_attention(
         q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0],
         os[1], None if lse is None else lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), n - 1, tq, tk, hq, hkv, d,
-        d ** -0.5 if scale is None else scale, 1 if causal else 0, _stream(dev))
+        d ** -0.5 if scale is None else scale, 1 if causal else 0, ws_ptr, ws_n, stream)
     _lib.check(st, "fp8gq_prompt_attention")
     return (out, lse) if return_lse else out
 

@@ -34,7 +34,7 @@ def decode(lib, c=None, q=A, qt=512, qh=128, table=A, ldt=8, pages=8, lens=A, ou
 
 def prompt(lib, q=A, qt=512, qh=128, k=A, kt=256, kh=128, cu=A, b=1, tq=9, tk=9, hq=4, hkv=2, d=128):
     return lib.fp8gq_prompt_attention(q, qt, qh, k, kt, kh, A, 256, 128, A, 512, 128, None, cu, A, b, tq, tk, hq, hkv, d,
-                                      0.1, 1, None)
+                                      0.1, 1, A, 1 << 20, None)
 
 
 def score(lib, x=A, ld=100, dtype=1 * 2, tok=A, t=3, v=100, lp=A, ids=A, tops=A, k=5):
