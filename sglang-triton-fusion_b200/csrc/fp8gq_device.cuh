@@ -135,6 +135,23 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, u
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// The same bounded wait for chains of short waits: the clock is first read after
+// 256 polls (reading it takes as long as such a wait).
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, unsigned int site) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 255u) == 0u) {
+      const uint64_t t = global_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > wait_limit_ns()) {
+        record_error(site);
+        return false;
+      }
+    }
+  }
+}
+
 // Bulk copy of `bytes` (multiple of 16, both addresses 16-byte aligned) from
 // global to this CTA's shared memory; completion is counted on `bar`.  The
 // weight stream is read once, so it is marked evict-first in L2.

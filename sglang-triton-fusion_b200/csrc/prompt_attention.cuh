@@ -139,6 +139,12 @@ __device__ __forceinline__ float ex2f(float x) {
   return y;
 }
 
+// A bounded wait, by one thread, or by all lanes of a warp with one outcome.
+__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity) { return mbar_wait_short(bar, parity, kSitePrompt); }
+__device__ __forceinline__ bool pr_wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, pr_wait(bar, parity)) != 0;
+}
+
 // An item: two query tiles of one sequence and kv head.
 struct PrWork {
   int q0, lq, k0, lk;       // the sequence's tokens (q0 < 0: no more items)
@@ -212,7 +218,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
   int item = 0;
   PrWork w;
   auto next_item = [&]() {
-    ok = mbar_wait_warp(&b_item[item % kPrItems], (item / kPrItems) & 1, kSitePrompt, lane) && ok;
+    ok = pr_wait_warp(&b_item[item % kPrItems], (item / kPrItems) & 1) && ok;
     if (!ok) return false;
     w = s_work[item % kPrItems];
     return w.q0 >= 0;
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             at += nb;
           }
         }
-        if (it >= kPrItems) ok = mbar_wait_warp(&b_taken[it % kPrItems], (it / kPrItems - 1) & 1, kSitePrompt, lane);
+        if (it >= kPrItems) ok = pr_wait_warp(&b_taken[it % kPrItems], (it / kPrItems - 1) & 1);
         if (!ok) break;
         if (here || (lane == 0 && id >= total)) s_work[it % kPrItems] = x;
         __syncwarp();
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         if (id >= total) break;
         // not before this item's loads are issued: an item taken early is one that
         // an idle CTA cannot take
-        ok = mbar_wait_warp(&b_want, it & 1, kSitePrompt, lane);
+        ok = pr_wait_warp(&b_want, it & 1);
         if (!ok) break;
         if (lane == 0) id = gridDim.x + atomicAdd(p.counters, 1);
         id = __shfl_sync(0xffffffffu, id, 0);
@@ -316,7 +322,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         const bool partial = n * kKeys > w.lk;      // the last tile reaches past the sequence
         if (n > 0) {
           if (lane == 0) {
-            if (items > 0) ok = mbar_wait(&b_qfree, (items - 1) & 1, kSitePrompt);
+            if (items > 0) ok = pr_wait(&b_qfree, (items - 1) & 1);
             if (ok) {
               mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
               for (int i = 0; i < 2; ++i)
@@ -325,7 +331,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             }
             for (int i = 0; i < 2 * n && ok; ++i) {            // k and v tiles in turn
               const int x = x0 + i, slot = x % kSlots;
-              if (x >= kSlots) ok = mbar_wait(&b_free[slot], (x / kSlots - 1) & 1, kSitePrompt);
+              if (x >= kSlots) ok = pr_wait(&b_free[slot], (x / kSlots - 1) & 1);
               if (!ok) break;
               uint64_t* bar = partial && i == 2 * n - 1 ? &b_tail : &b_full[slot];
               mbar_arrive_expect_tx(bar, kTile);
@@ -338,7 +344,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
           if (partial) {
             // rows past the sequence: zeros, then the tile is there
             const int slot = (x0 + 2 * n - 1) % kSlots, valid = w.lk - (n - 1) * kKeys;
-            ok = mbar_wait_warp(&b_tail, tails & 1, kSitePrompt, lane);
+            ok = pr_wait_warp(&b_tail, tails & 1);
             if (!ok) break;
             for (int x = valid * 8 + lane; x < kKeys * 8; x += 32)
               for (int h = 0; h < Cfg::kHalves; ++h)
@@ -359,8 +365,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       // the copies that no one has waited for have landed before the CTA ends
       // (only after a wait gave up: otherwise every tile has been used)
       if (!ok && lane == 0) {
-        mbar_wait(&b_q, items & 1, kSitePrompt);
-        for (int i = 0; i < kSlots; ++i) mbar_wait(&b_full[i], (x0 / kSlots) & 1, kSitePrompt);
+        pr_wait(&b_q, items & 1);
+        for (int i = 0; i < kSlots; ++i) pr_wait(&b_full[i], (x0 / kSlots) & 1);
       }
     } else {
       // ---- MMA of tile i ----
@@ -371,10 +377,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       while (next_item()) {
         const int mine = w.n[i], n = max(w.n[0], w.n[1]);
         if (n > 0 && lane == 0) {
-          auto full = [&](int x) { return mbar_wait(&b_full[x % kSlots], (x / kSlots) & 1, kSitePrompt); };
+          auto full = [&](int x) { return pr_wait(&b_full[x % kSlots], (x / kSlots) & 1); };
           auto scores = [&](int j) {                       // S = Q K^T of tile j
             const int x = x0 + 2 * j, step = step0 + j;
-            ok = full(x) && (step == 0 || mbar_wait(&b_r[i], (step - 1) & 1, kSitePrompt));
+            ok = full(x) && (step == 0 || pr_wait(&b_r[i], (step - 1) & 1));
             if (!ok) return;
             tc_fence_after();
             const uint32_t a = base + i * Cfg::kQTile, b = ring + (x % kSlots) * kTile;
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             mma_commit(&b_s[i]);
             mma_commit(&b_free[x % kSlots]);
           };
-          ok = mbar_wait(&b_q, items & 1, kSitePrompt);
+          ok = pr_wait(&b_q, items & 1);
           if (ok && mine > 0) scores(0);
           for (int j = 0; j < mine && ok; ++j) {
             if (j + 1 < mine) {
@@ -394,8 +400,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             }
             if (j + 1 >= mine) mma_commit(&b_qfree);                     // q has been read
             const int x = x0 + 2 * j + 1;
-            ok = full(x) && mbar_wait(&b_p[i], (step0 + j) & 1, kSitePrompt) &&
-                 (j > 0 || outs == 0 || mbar_wait(&b_out[i], (outs - 1) & 1, kSitePrompt));
+            ok = full(x) && pr_wait(&b_p[i], (step0 + j) & 1) &&
+                 (j > 0 || outs == 0 || pr_wait(&b_out[i], (outs - 1) & 1));
             if (!ok) break;
             tc_fence_after();
             const uint32_t b = ring + (x % kSlots) * kTile;              // O += P V
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       }
       if (!ok && lane == 0) {                              // what has been issued completes
         mma_commit(&b_o[i]);
-        mbar_wait(&b_o[i], step0 & 1, kSitePrompt);
+        pr_wait(&b_o[i], step0 & 1);
       }
     }
   } else {
@@ -442,7 +448,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < mine; ++j) {
         const int step = step0 + j;
-        ok = mbar_wait_warp(&b_s[i], step & 1, kSitePrompt, lane);
+        ok = pr_wait_warp(&b_s[i], step & 1);
         if (!ok) break;
         tc_fence_after();
         uint32_t s[kKeys];
@@ -475,7 +481,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
           const float mn = fmaxf(m, mx);
           if (j > 0) {
             // (the products of the tile before have updated O)
-            ok = mbar_wait_warp(&b_o[i], (step - 1) & 1, kSitePrompt, lane);
+            ok = pr_wait_warp(&b_o[i], (step - 1) & 1);
             if (!ok) break;
             tc_fence_after();
             const float a = m == -INFINITY ? 0.0f : ex2f((m - mn) * c);
@@ -513,7 +519,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
           }
           if (x == 0 && step > 0) {
             // the products of the tile before have read P by now
-            ok = mbar_wait_warp(&b_o[i], (step - 1) & 1, kSitePrompt, lane);
+            ok = pr_wait_warp(&b_o[i], (step - 1) & 1);
             if (!ok) break;
             tc_fence_after();
           }
@@ -531,7 +537,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       if (!ok) break;
       step0 += mine;
       if (mine > 0) {
-        ok = mbar_wait_warp(&b_o[i], (step0 - 1) & 1, kSitePrompt, lane);
+        ok = pr_wait_warp(&b_o[i], (step0 - 1) & 1);
         if (!ok) break;
         tc_fence_after();
       }
