@@ -139,6 +139,16 @@ __device__ __forceinline__ float ex2f(float x) {
   return y;
 }
 
+// One lane of the (converged) warp.  tcgen05.mma takes its operands from uniform
+// registers; behind a branch on the lane number the compiler issues it lane by
+// lane, 114 cycles each, whatever its size (70 to 87 behind this one at 128 x 128
+// x 16).
+__device__ __forceinline__ bool pr_elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // A bounded wait, by one thread, or by all lanes of a warp with one outcome.
 __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity) { return mbar_wait_short(bar, parity, kSitePrompt); }
 __device__ __forceinline__ bool pr_wait_warp(uint64_t* bar, uint32_t parity) {
@@ -321,25 +331,27 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         const int n = max(w.n[0], w.n[1]);
         const bool partial = n * kKeys > w.lk;      // the last tile reaches past the sequence
         if (n > 0) {
-          if (lane == 0) {
-            if (items > 0) ok = pr_wait(&b_qfree, (items - 1) & 1);
-            if (ok) {
-              mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
-              for (int i = 0; i < 2; ++i)
-                for (int h = 0; h < Cfg::kHalves; ++h)
-                  tma_load_3d(base + i * Cfg::kQTile + h * 16384, &tq, 64 * h, w.hk * p.group, w.q0 + w.r0 + i * p.rows, &b_q);
-            }
-            for (int i = 0; i < 2 * n && ok; ++i) {            // k and v tiles in turn
-              const int x = x0 + i, slot = x % kSlots;
-              if (x >= kSlots) ok = pr_wait(&b_free[slot], (x / kSlots - 1) & 1);
-              if (!ok) break;
+          if (items > 0) ok = pr_wait_warp(&b_qfree, (items - 1) & 1);
+          if (!ok) break;
+          if (pr_elect()) {
+            mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
+            for (int i = 0; i < 2; ++i)
+              for (int h = 0; h < Cfg::kHalves; ++h)
+                tma_load_3d(base + i * Cfg::kQTile + h * 16384, &tq, 64 * h, w.hk * p.group, w.q0 + w.r0 + i * p.rows, &b_q);
+          }
+          __syncwarp();
+          for (int i = 0; i < 2 * n; ++i) {                    // k and v tiles in turn
+            const int x = x0 + i, slot = x % kSlots;
+            if (x >= kSlots) ok = pr_wait_warp(&b_free[slot], (x / kSlots - 1) & 1);
+            if (!ok) break;
+            if (pr_elect()) {
               uint64_t* bar = partial && i == 2 * n - 1 ? &b_tail : &b_full[slot];
               mbar_arrive_expect_tx(bar, kTile);
               for (int h = 0; h < Cfg::kHalves; ++h)
                 tma_load_3d(ring + slot * kTile + h * Cfg::kHalf, (i & 1) ? &tv : &tk, 64 * h, w.hk, w.k0 + (i >> 1) * kKeys, bar);
             }
+            __syncwarp();
           }
-          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
           if (!ok) break;
           if (partial) {
             // rows past the sequence: zeros, then the tile is there
@@ -369,65 +381,73 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         for (int i = 0; i < kSlots; ++i) pr_wait(&b_full[i], (x0 / kSlots) & 1);
       }
     } else {
-      // ---- MMA of tile i ----
-      const int i = warp - 9;
+      // ---- MMA of tile i: the warp waits together, one lane issues ----
+      const int i = __shfl_sync(0xffffffffu, warp, 0) - 9;
       const uint32_t id_s = pr_idesc(kKeys, false, p.negate != 0), id_o = pr_idesc(D, true, false);
-      const uint32_t ts = tmem + Cfg::kS + i * kKeys, tp = tmem + Cfg::kP + i * Cfg::kPCols, to = tmem + i * D;
+      const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t ts = t0 + Cfg::kS + i * kKeys, tp = t0 + Cfg::kP + i * Cfg::kPCols, to = t0 + i * D;
       int x0 = 0, items = 0, step0 = 0, outs = 0;   // tiles, items with tiles, this tile's steps and outputs so far
+      auto full = [&](int x) { return pr_wait_warp(&b_full[x % kSlots], (x / kSlots) & 1); };
+      auto scores = [&](int j) {                           // S = Q K^T of tile j
+        const int x = x0 + 2 * j, step = step0 + j;
+        ok = full(x) && (step == 0 || pr_wait_warp(&b_r[i], (step - 1) & 1));
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t a = base + i * Cfg::kQTile, b = ring + (x % kSlots) * kTile;
+        if (pr_elect()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(ts, pr_desc(a + (k >> 2) * 16384 + (k & 3) * 32, 16), pr_desc(b + (k >> 2) * Cfg::kHalf + (k & 3) * 32, 16),
+                   id_s, k > 0);
+          mma_commit(&b_s[i]);
+          mma_commit(&b_free[x % kSlots]);
+        }
+        __syncwarp();
+      };
       while (next_item()) {
         const int mine = w.n[i], n = max(w.n[0], w.n[1]);
-        if (n > 0 && lane == 0) {
-          auto full = [&](int x) { return pr_wait(&b_full[x % kSlots], (x / kSlots) & 1); };
-          auto scores = [&](int j) {                       // S = Q K^T of tile j
-            const int x = x0 + 2 * j, step = step0 + j;
-            ok = full(x) && (step == 0 || pr_wait(&b_r[i], (step - 1) & 1));
-            if (!ok) return;
-            tc_fence_after();
-            const uint32_t a = base + i * Cfg::kQTile, b = ring + (x % kSlots) * kTile;
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              mma_ss(ts, pr_desc(a + (k >> 2) * 16384 + (k & 3) * 32, 16), pr_desc(b + (k >> 2) * Cfg::kHalf + (k & 3) * 32, 16),
-                     id_s, k > 0);
-            mma_commit(&b_s[i]);
-            mma_commit(&b_free[x % kSlots]);
-          };
-          ok = pr_wait(&b_q, items & 1);
+        if (n > 0) {
+          ok = pr_wait_warp(&b_q, items & 1);
           if (ok && mine > 0) scores(0);
           for (int j = 0; j < mine && ok; ++j) {
-            if (j + 1 < mine) {
+            const bool more = j + 1 < mine;
+            if (more) {
               scores(j + 1);
               if (!ok) break;
             }
-            if (j + 1 >= mine) mma_commit(&b_qfree);                     // q has been read
             const int x = x0 + 2 * j + 1;
-            ok = full(x) && pr_wait(&b_p[i], (step0 + j) & 1) &&
-                 (j > 0 || outs == 0 || pr_wait(&b_out[i], (outs - 1) & 1));
+            ok = full(x) && (j > 0 || outs == 0 || pr_wait_warp(&b_out[i], (outs - 1) & 1)) &&
+                 pr_wait_warp(&b_p[i], (step0 + j) & 1);
             if (!ok) break;
             tc_fence_after();
             const uint32_t b = ring + (x % kSlots) * kTile;              // O += P V
+            if (pr_elect()) {
+              if (!more) mma_commit(&b_qfree);                           // q has been read
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, tp + 8 * k, pr_desc(b + k * 2048, Cfg::kHalf), id_o, j > 0 || k > 0);
-            mma_commit(&b_free[x % kSlots]);
-            mma_commit(&b_o[i]);                                         // (the last commit of an item)
+              for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, tp + 8 * k, pr_desc(b + k * 2048, Cfg::kHalf), id_o, j > 0 || k > 0);
+              mma_commit(&b_free[x % kSlots]);
+              mma_commit(&b_o[i]);                                       // (the last commit of an item)
+            }
+            __syncwarp();
           }
-          if (mine == 0) mbar_arrive(&b_qfree);
+          if (mine == 0 && ok && lane == 0) mbar_arrive(&b_qfree);
           // the tiles that only the other query tile sees
           for (int x = 2 * mine; x < 2 * n && ok; ++x) {
             ok = full(x0 + x);
-            if (ok) mbar_arrive(&b_free[(x0 + x) % kSlots]);
+            if (ok && lane == 0) mbar_arrive(&b_free[(x0 + x) % kSlots]);
           }
+          ++items;
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (!ok) break;
-        if (n > 0) ++items;
         x0 += 2 * n;
         step0 += mine;
         if (mine > 0) ++outs;
         leave_item();
       }
-      if (!ok && lane == 0) {                              // what has been issued completes
-        mma_commit(&b_o[i]);
-        pr_wait(&b_o[i], step0 & 1);
+      if (!ok) {                                           // what has been issued completes
+        if (pr_elect()) mma_commit(&b_o[i]);
+        __syncwarp();
+        pr_wait_warp(&b_o[i], step0 & 1);
       }
     }
   } else {
