@@ -27,6 +27,10 @@
 // written.  (A CTA per item spent 13000 cycles of its own before and after its
 // tiles: as much as 6 tiles take.)
 //
+// The two tiles' warps that share a scheduler take turns at the exponentials:
+// left alone they fall into step, both in the MUFU at half speed and then both
+// waiting (1 x 8192: XXX against 526 us).
+//
 // Warps 0-3 and 4-7: softmax, output (one thread per row of tile 0, 1).  Warp 8:
 // TMA; it also clears the rows of the last v tile that lie past the sequence
 // (another sequence's values, which a weight of 0 does not stop if they are
@@ -178,6 +182,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
   __shared__ uint64_t b_full[kSlots], b_free[kSlots];
   __shared__ uint64_t b_s[2], b_r[2], b_p[2], b_o[2];        // scores ready, read; weights ready; O updated
   __shared__ uint64_t b_out[2];                              // O read
+  __shared__ uint64_t b_turn[2][4];                          // tile i's warp may have the MUFU
   __shared__ uint32_t s_tmem;
   __shared__ PrWork s_work[kPrItems];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -208,6 +213,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         mbar_init(&b_p[i], 4);
         mbar_init(&b_o[i], 1);
         mbar_init(&b_out[i], 4);
+        for (int x = 0; x < 4; ++x) mbar_init(&b_turn[i][x], 1);
       }
       fence_mbar_init();
     }
@@ -458,7 +464,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
     const uint32_t ts = lanes + Cfg::kS + i * kKeys, tp = lanes + Cfg::kP + i * Cfg::kPCols, to = lanes + i * D;
     const uint32_t stage = out_stage + warp * 4096;        // 32 rows of 64 values
     const float c = p.scale_log2;
-    int step0 = 0;                                         // this tile's steps so far
+    int step0 = 0, turns = 0;                              // this tile's steps so far, the turns of both
+    auto take_turn = [&]() { return (i == 0 && turns == 0) || pr_wait_warp(&b_turn[i][warp & 3], (turns - 1 + i) & 1); };
+    auto pass_turn = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b_turn[1 - i][warp & 3]);
+      ++turns;
+    };
     while (next_item()) {
       const int mine = w.n[i];
       const int tok = w.r0 + i * p.rows + row_tok;         // token within the sequence
@@ -525,6 +537,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         float2 sum[4];
 #pragma unroll
         for (int y = 0; y < 4; ++y) sum[y] = make_float2(0.0f, 0.0f);
+        if (step > 0) {
+          // the products of the tile before have read P by now
+          ok = pr_wait_warp(&b_o[i], (step - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        ok = take_turn();
+        if (!ok) break;
         constexpr int kPart = kKeys > 80 ? kKeys / 2 : kKeys;          // (registers)
 #pragma unroll
         for (int x = 0; x < kKeys; x += kPart) {
@@ -537,22 +557,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
             q[y] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          if (x == 0 && step > 0) {
-            // the products of the tile before have read P by now
-            ok = pr_wait_warp(&b_o[i], (step - 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-          }
 #pragma unroll
           for (int y = 0; y < kPart / 2; y += 8) tmem_st8(tp + x / 2 + y, q + y);
         }
-        if (!ok) break;
+        pass_turn();
         const float2 sum2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
         l += sum2.x + sum2.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&b_p[i]);
+      }
+      for (int j = mine; j < max(w.n[0], w.n[1]) && ok; ++j) {       // the other tile's last turns
+        ok = take_turn();
+        pass_turn();
       }
       if (!ok) break;
       step0 += mine;
