@@ -29,7 +29,9 @@
 //
 // The two tiles' warps that share a scheduler take turns at the exponentials:
 // left alone they fall into step, both in the MUFU at half speed and then both
-// waiting (1 x 8192: XXX against 526 us).
+// waiting (1 x 8192: 453 against 526 us).  Computing a part of them on the fma
+// pipe instead (2^n times a polynomial) was slower at every part: the two warps
+// of a scheduler have no issue slots to spare.
 //
 // Warps 0-3 and 4-7: softmax, output (one thread per row of tile 0, 1).  Warp 8:
 // TMA; it also clears the rows of the last v tile that lie past the sequence
@@ -142,6 +144,8 @@ __device__ __forceinline__ float ex2f(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+constexpr int kPassAfter = 2;      // 16-key chunks after which the turn is passed
 
 // One lane of the (converged) warp.  tcgen05.mma takes its operands from uniform
 // registers; behind a branch on the lane number the compiler issues it lane by
@@ -545,22 +549,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         }
         ok = take_turn();
         if (!ok) break;
-        constexpr int kPart = kKeys > 80 ? kKeys / 2 : kKeys;          // (registers)
 #pragma unroll
-        for (int x = 0; x < kKeys; x += kPart) {
-          uint32_t q[kPart / 2];
+        for (int x = 0; x < kKeys; x += 16) {
+          uint32_t q[8];
 #pragma unroll
-          for (int y = 0; y < kPart / 2; ++y) {
+          for (int y = 0; y < 8; ++y) {
             const float2 t = fma2(make_float2(__uint_as_float(s[x + 2 * y]), __uint_as_float(s[x + 2 * y + 1])), c2, mc2);
             const float2 e = make_float2(ex2f(t.x), ex2f(t.y));
             sum[y & 3] = add2(sum[y & 3], e);
             const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
             q[y] = *reinterpret_cast<const uint32_t*>(&h);
           }
-#pragma unroll
-          for (int y = 0; y < kPart / 2; y += 8) tmem_st8(tp + x / 2 + y, q + y);
+          tmem_st8(tp + x / 2, q);
+          if (x / 16 == kPassAfter) pass_turn();           // (the hand-over takes as long as the rest)
         }
-        pass_turn();
         const float2 sum2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
         l += sum2.x + sum2.y;
         tmem_wait_st();
