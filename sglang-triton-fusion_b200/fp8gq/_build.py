@@ -1,5 +1,5 @@
 """Build libfp8gq.so (the C ABI in include/fp8gq.h) in-tree with nvcc for
-sm_100a.  Run ``python -m fp8gq._build`` (with ``sglang-triton-fusion_b200``
+sm_100a, and the serving operators' Python binding next to it with g++.  Run ``python -m fp8gq._build`` (with ``sglang-triton-fusion_b200``
 on sys.path) or call :func:`build`."""
 from __future__ import annotations
 
@@ -19,6 +19,8 @@ HEADERS = {"fp8gq_api.cu": ["fp8gq_device.cuh", "host_common.h", "tensor_core.cu
            "serve_api.cu": ["fp8gq_device.cuh", "host_common.h", "tensor_core.cuh", "rope_append.cuh",
                             "paged_decode.cuh", "prompt_attention.cuh", "token_logprobs.cuh"]}
 OBJ_DIR = PKG_DIR / "build"
+NATIVE_SOURCE = "serve_python.cpp"               # the serving operators' Python binding
+NATIVE_PATH = PKG_DIR / "_serve_native.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -46,8 +48,28 @@ def _newer_than(target: Path, files) -> bool:
     return all(f.stat().st_mtime <= t for f in files)
 
 
+def _native_inputs():
+    return [SRC_DIR / NATIVE_SOURCE, REPO_DIR / "include" / "fp8gq.h"]
+
+
 def up_to_date() -> bool:
-    return _newer_than(LIB_PATH, [f for s in SOURCES for f in _inputs(s)])
+    return _newer_than(LIB_PATH, [f for s in SOURCES for f in _inputs(s)]) and _newer_than(NATIVE_PATH, _native_inputs())
+
+
+def _native_command(target: str):
+    """g++ command of the binding, which links torch's libraries (loaded by then)
+    and libfp8gq.so next to it."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    inc = [*include_paths(), sysconfig.get_paths()["include"], str(REPO_DIR / "include"),
+           str(Path(nvcc_path()).resolve().parent.parent / "include")]
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{i}" for i in inc],
+            str(SRC_DIR / NATIVE_SOURCE), "-o", target, f"-L{PKG_DIR}", "-l:libfp8gq.so",
+            f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
@@ -78,6 +100,11 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     os.replace(str(LIB_PATH) + ".tmp", LIB_PATH)
+    if force or not _newer_than(NATIVE_PATH, _native_inputs()):
+        res = subprocess.run(_native_command(str(NATIVE_PATH) + ".tmp"), capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        os.replace(str(NATIVE_PATH) + ".tmp", NATIVE_PATH)
     return LIB_PATH
 
 

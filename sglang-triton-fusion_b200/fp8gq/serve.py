@@ -15,12 +15,14 @@ recorded in the device error word (``device_error()``), not raised.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 from typing import NamedTuple
 
 import torch
 
-from . import _lib
-from .ops import RMS_EPS, ShapeError, _check_cuda, _stream, _workspace_entry
+from . import _build, _lib
+from .ops import RMS_EPS, ShapeError, _check_cuda, _stream, _workspace_entry, _workspaces
 
 HEAD_DIMS = (64, 128)
 MAX_TOP = 32
@@ -28,6 +30,25 @@ PROMPT_WORKSPACE = 16   # fp8gq_prompt_workspace_bytes()
 _BF16, _E4M3, _F32 = 0, 1, 2   # FP8GQ_DTYPE_*
 _byref = ctypes.byref
 _decode_ws_bytes: dict = {}    # (device, Hq, Hkv, D) -> fp8gq_paged_decode_workspace_bytes
+
+
+class _Binding:
+    """The C++ binding (csrc/serve_python.cpp), loaded at the first call.  Its
+    functions return None for anything but the plain form of the arguments; the
+    checks below then raise, or complete the call."""
+
+    def __getattr__(self, name):
+        _lib.load()
+        loader = importlib.machinery.ExtensionFileLoader("_serve_native", str(_build.NATIVE_PATH))
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_serve_native", loader))
+        loader.exec_module(mod)
+        mod.set_workspaces(_workspaces)
+        global _native
+        _native = mod
+        return getattr(mod, name)
+
+
+_native = _Binding()
 
 
 def _check_cache(k, v, k_scale, v_scale):
@@ -84,6 +105,11 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch
     place; negative: not stored).  ``return_k`` also returns k (T, Hkv, D) as it
     is before the cache's rounding to e4m3, for prompt_attention.  ``q_out`` and
     ``k_out`` may be views of qkv."""
+    if q_out is None and k_out is None:
+        r = _native.qk_norm_rope_append(qkv, positions, slots, cos_sin, k_cache, v_cache, q_weight, k_weight, eps,
+                                        k_scale, v_scale, return_k)
+        if r is not None:
+            return r
     _check_cuda(qkv, positions, slots, cos_sin, k_cache, v_cache, q_weight, k_weight, q_out, k_out)
     cache, hkv, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.stride(1) != 1:
@@ -123,6 +149,10 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     ``scale`` is 1 / sqrt(D) by default.  Hq is a multiple of the cache's heads.
     A sequence of length 0 gives 0.  ``return_lse`` also returns the log of the
     softmax's sum, fp32 (B, Hq)."""
+    if out is None:
+        r = _native.paged_decode_attention(q, k_cache, v_cache, page_table, lens, scale, k_scale, v_scale, return_lse)
+        if r is not None:
+            return r
     _check_cuda(q, k_cache, v_cache, page_table, lens, out)
     cache, hkv, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
     (b, hq, _), qs = _check_heads(q, "q", d)
@@ -165,6 +195,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     j <= i + (k tokens - q tokens), so that its last row sees all of them.  A row
     that sees none gives 0; rows past cu_q[B] are not written.  ``scale`` is
     1 / sqrt(D) by default.  ``return_lse`` also returns fp32 (Tq, Hq)."""
+    if out is None:
+        r = _native.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)
+        if r is not None:
+            return r
     _check_cuda(q, k, v, cu_q, cu_k, out)
     (tq, hq, d), qs = _check_heads(q, "q")
     (tk, hkv, _), ks = _check_heads(k, "k", d)
@@ -212,6 +246,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     [T]; negative: none given, 0), the entropy and the ``top_k`` <= 32 likeliest
     tokens of each row (equal logits by ascending index).  -inf rules a token
     out; a row with NaN or +inf, or with no finite logit, has NaN throughout."""
+    r = _native.token_logprobs(logits, tokens, top_k)
+    if r is not None:
+        return TokenLogprobs._make(r)
     _check_cuda(logits, tokens)
     if logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2:
         raise TypeError("logits must be a 2-D bf16 or fp32 tensor")
