@@ -38,7 +38,9 @@ struct AppendParams {
   __nv_bfloat16* k_out;
   int64_t ldk;
   CacheView cache;
-  int T, Hq, Hkv;
+  uint32_t units;           // T * (Hq + 2 Hkv)
+  int Hq, Hkv;
+  int page_shift;           // log2(page_size), or -1
 };
 
 constexpr int kAppendThreads = 256;
@@ -76,20 +78,24 @@ template <int D, bool kFp8>
 __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const AppendParams p) {
   constexpr int L = D / 16;              // lanes per head
   grid_dependency_wait();
-  const int heads = p.Hq + 2 * p.Hkv;
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x) / L;
+  const uint32_t heads = p.Hq + 2 * p.Hkv;
+  const uint32_t unit = blockIdx.x * (kAppendThreads / L) + threadIdx.x / L;       // (token, head)
   const int l = threadIdx.x % L;
-  const bool live = unit < static_cast<int64_t>(p.T) * heads;
+  const bool live = unit < p.units;
   // lanes past the end follow the last unit through the shuffles and store nothing
-  const int64_t u = live ? unit : static_cast<int64_t>(p.T) * heads - 1;
-  const int64_t t = u / heads;
-  const int h = static_cast<int>(u - t * heads);
+  const uint32_t u = live ? unit : p.units - 1;
+  const uint32_t tok = u / heads;
+  const int64_t t = tok;
+  const int h = static_cast<int>(u - tok * heads);
   const __nv_bfloat16* src = p.qkv + t * p.ldqkv + static_cast<int64_t>(h) * D + 8 * l;
-  float a[8], b[8];
-  unpack8(a, *reinterpret_cast<const uint4*>(src));
-  unpack8(b, *reinterpret_cast<const uint4*>(src + D / 2));
   const bool is_q = h < p.Hq;
   const bool is_v = h >= p.Hq + p.Hkv;
+  const uint4 lo = __ldcs(reinterpret_cast<const uint4*>(src)), hi = __ldcs(reinterpret_cast<const uint4*>(src + D / 2));
+  const int64_t position = is_v ? 0 : __ldg(p.positions + t);
+  const int64_t slot = is_q ? -1 : __ldg(p.slots + t);
+  float a[8], b[8];
+  unpack8(a, lo);
+  unpack8(b, hi);
   const __nv_bfloat16* w = is_v ? nullptr : is_q ? p.qw : p.kw;
   float ss = 0.0f;
 #pragma unroll
@@ -97,7 +103,7 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (w) {
-    const float rstd = 1.0f / sqrtf(ss / D + p.eps);
+    const float rstd = rsqrtf(ss * (1.0f / D) + p.eps);
     float wa[8], wb[8];
     unpack8(wa, *reinterpret_cast<const uint4*>(w + 8 * l));
     unpack8(wb, *reinterpret_cast<const uint4*>(w + D / 2 + 8 * l));
@@ -108,7 +114,7 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
     }
   }
   if (!is_v) {
-    int64_t pos = p.positions[t];
+    int64_t pos = position;
     if (pos < 0 || pos >= p.max_position) {
       record_error(kSiteBadIndex);
       pos = pos < 0 ? 0 : p.max_position - 1;
@@ -131,17 +137,16 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const Appen
       *reinterpret_cast<uint4*>(o) = pack8(a);
       *reinterpret_cast<uint4*>(o + D / 2) = pack8(b);
     } else {
-      const int hk = (h - p.Hq) % p.Hkv;
+      const int hk = is_v ? h - p.Hq - p.Hkv : h - p.Hq;
       if (!is_v && p.k_out) {
         __nv_bfloat16* o = p.k_out + t * p.ldk + static_cast<int64_t>(hk) * D + 8 * l;
         *reinterpret_cast<uint4*>(o) = pack8(a);
         *reinterpret_cast<uint4*>(o + D / 2) = pack8(b);
       }
-      const int64_t slot = p.slots[t];
       if (slot >= p.cache.num_pages * p.cache.page_size) {
         record_error(kSiteBadIndex);
       } else if (slot >= 0) {
-        const int64_t page = slot / p.cache.page_size;
+        const int64_t page = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.cache.page_size;
         const int64_t at = slot - page * p.cache.page_size;
         const int64_t off = (is_v ? page * p.cache.v_page + at * p.cache.v_slot + hk * p.cache.v_head
                                   : page * p.cache.k_page + at * p.cache.k_slot + hk * p.cache.k_head) + 8 * l;

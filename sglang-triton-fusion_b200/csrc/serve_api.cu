@@ -39,6 +39,13 @@ int check_heads(int Hq, int Hkv, int D) {
   return FP8GQ_OK;
 }
 
+// log2 of a power of two, -1 of any other number.
+int log2_of(int x) {
+  for (int i = 0; i < 31; ++i)
+    if (x == 1 << i) return i;
+  return -1;
+}
+
 // A cache's checks; strides are multiples of 16 bytes and (for a cache with
 // several pages, slots or heads) positive.
 int to_cache_view(const fp8gq_paged_cache* c, int Hkv, int D, CacheView* v) {
@@ -175,12 +182,13 @@ int fp8gq_qk_norm_rope_append(const void* qkv, int64_t ldqkv, const int64_t* pos
   p.ldq = ldq;
   p.k_out = static_cast<__nv_bfloat16*>(k_out);
   p.ldk = ldk;
-  p.T = T;
   p.Hq = Hq;
   p.Hkv = Hkv;
-  const int64_t threads = static_cast<int64_t>(T) * heads * (D / 16);
-  const int64_t blocks = (threads + kAppendThreads - 1) / kAppendThreads;
-  if (blocks > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
+  p.page_shift = log2_of(cache->page_size);
+  const int64_t units = static_cast<int64_t>(T) * heads, per_block = kAppendThreads / (D / 16);
+  const int64_t blocks = (units + per_block - 1) / per_block;
+  if (units > INT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
+  p.units = static_cast<uint32_t>(units);
   const bool fp8 = cache->dtype == FP8GQ_DTYPE_E4M3;
   auto fn = D == 128 ? (fp8 ? rope_append_kernel<128, true> : rope_append_kernel<128, false>)
                      : (fp8 ? rope_append_kernel<64, true> : rope_append_kernel<64, false>);
@@ -238,9 +246,7 @@ int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t 
                          (Hkv - 1) * (kv ? cache->v_head_stride : cache->k_head_stride) + D;
     if (span / (fp8 ? 16 : 8) > UINT32_MAX) return FP8GQ_ERR_UNSUPPORTED;
   }
-  p.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (cache->page_size == 1 << i) p.page_shift = i;
+  p.page_shift = log2_of(cache->page_size);
   p.group = Hq / Hkv;
   const int nt = p.group > 8 ? 2 : 1;
   p.blocks = (p.group + 8 * nt - 1) / (8 * nt);
