@@ -9,7 +9,7 @@
 //
 // Work split: the tiles (4 warps x kTok tokens of one sequence and kv head) of
 // all sequences form one flat list, cut into equal contiguous ranges, one per
-// CTA, two CTAs per SM; the start of each (sequence, head) counts as
+// CTA, two or four CTAs per SM; the start of each (sequence, head) counts as
 // kDecItemCost tiles more.  The lengths are read on the device (a captured step
 // replays while they grow), so ragged batches and long single sequences
 // balance the same way.  A (sequence, head) that lies in several ranges leaves
@@ -17,13 +17,17 @@
 // order, so the result does not depend on who is last.
 //
 // Inside a CTA each warp runs alone: its lanes look up the pages of its own
-// kTok tokens and copy their rows of k and v (8 KB per step, kDecStages steps in
+// kTok tokens and copy their rows of k and v (4 or 8 KB per step, kDecStages steps in
 // flight), and it computes on them with matrix instructions whose M side is the
 // tokens (S^T = K Q^T, 16 x 8) and then the head's values (O^T = V^T P^T), so a
 // group of up to 8 query heads wastes nothing of K and V and no barrier stands
 // in the loop.  The copies are 16-byte cp.async: any page size and stride, and
 // one bulk copy per row was measured at 16 cycles each (8 x 32768 tokens, e4m3:
-// 235 us against 131).
+// 235 us against 131 as the rest stood then).
+//
+// Measured, 32 query and 8 kv heads of 128: 64 x 4096 tokens 179 us (6.0 TB/s),
+// 48 ragged to 6000 72 us (5.5 TB/s), 8 x 32768 in e4m3 98 us (5.5 TB/s), 1 x 333
+// 8.6 us (the latency of one range and its join).
 #pragma once
 
 #include "fp8gq_device.cuh"
@@ -56,15 +60,24 @@ struct DecodeParams {
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecStages = 3;
-constexpr int kDecStepBytes = 8192;         // k and v rows of one warp's step
 constexpr int kDecCounterBytes = 16384;     // the workspace's counters (the tile kernel's too)
-constexpr int kDecMinTiles = 2;             // tiles per CTA below which fewer CTAs work
-constexpr int kDecItemCost = 1;             // what starting a (sequence, head) counts, in tiles
+// Tiles per CTA below which fewer CTAs work (1 x 333 and 1 x 2000 tokens: 1: 8.2
+// and 11.3 us; 2: 8.6 and 9.5; 3: 9.7 and 10.6).
+constexpr int kDecMinTiles = 2;
+// What starting a (sequence, head) counts, in tiles (48 ragged to 6000: 0: 108
+// us, 1: 75, 2: 71).
+constexpr int kDecItemCost = 2;
 
-template <int D, bool kFp8>
+template <int D, bool kFp8, int kNT>
 struct DecCfg {
+  // Two CTAs per SM of 8 KB steps; at 64 e4m3 values a head, four of 4 KB (128 x
+  // 2047 tokens, 2 kv heads: 39 against 45 us; the other kinds are slower that
+  // way: 8 x 32768 e4m3 at D = 128 186 against 98 us, 128 ragged bf16 at D = 64
+  // 30 against 21 us).
+  static constexpr int kCtas = D == 64 && kFp8 && kNT == 1 ? 4 : 2;
+  static constexpr int kStep = kCtas == 4 ? 4096 : 8192;      // bytes of k and v rows of one warp's step
   static constexpr int kRow = D * (kFp8 ? 1 : 2);       // bytes of a row
-  static constexpr int kTok = kDecStepBytes / 2 / kRow;
+  static constexpr int kTok = kStep / 2 / kRow;
   static constexpr int kTile = kTok * kDecWarps;
   static constexpr int kChunks = kRow / 16;
   // distance of rows in shared memory: rows read by one phase of a load fall on
@@ -187,8 +200,8 @@ struct DecWalk {
 };
 
 template <int D, bool kFp8, int kNT>
-__global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const DecodeParams p) {
-  using Cfg = DecCfg<D, kFp8>;
+__global__ void __launch_bounds__(kDecThreads, DecCfg<D, kFp8, kNT>::kCtas) paged_decode_kernel(const DecodeParams p) {
+  using Cfg = DecCfg<D, kFp8, kNT>;
   constexpr int kTok = Cfg::kTok, kTile = Cfg::kTile, kMT = D / 16, kKT = D / 16, kTT = kTok / 16;
   constexpr int kSlot = dec_slot_floats(D, kNT);
   constexpr int kRowK = Cfg::kRowK, kRowV = Cfg::kRowV;
@@ -246,13 +259,18 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
 
   const int64_t want = (total + kDecMinTiles - 1) / kDecMinTiles;
   const int64_t ctas = want < gridDim.x ? want : gridDim.x;
-  const int64_t t0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : 0;
-  const int64_t t1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : 0;
+  // x / y; 64-bit divisions take hundreds of cycles, and few lists need them
+  const bool narrow = (total + 1) * (ctas + 1) <= UINT32_MAX;
+  auto quotient = [&](int64_t x, int64_t y) {
+    return narrow ? static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y)) : x / y;
+  };
+  const int64_t t0 = blockIdx.x < ctas ? quotient(blockIdx.x * total, ctas) : 0;
+  const int64_t t1 = blockIdx.x < ctas ? quotient((blockIdx.x + 1) * total, ctas) : 0;
   if (t0 >= t1) {
     grid_launch_dependents();
     return;
   }
-  auto owner = [&](int64_t t) { return static_cast<int>(((t + 1) * ctas - 1) / total); };
+  auto owner = [&](int64_t t) { return static_cast<int>(quotient((t + 1) * ctas - 1, total)); };
 
   auto enter = [&](DecWalk& w) {              // w.b, w.sub and w.start are set
     w.n = (w.len + kTile - 1) / kTile;
@@ -295,7 +313,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
       at += here;
     }
     cur.b = b;
-    cur.sub = static_cast<int>((t0 - at) / per);
+    cur.sub = static_cast<int>(quotient(t0 - at, per));
     cur.start = at + static_cast<int64_t>(cur.sub) * per;
     enter(cur);
     if (!cur.done && cur.j >= cur.j_end) cur.done = true;      // (t1 lies before its first tile)
@@ -335,6 +353,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
   auto issue = [&](int stage) {
     constexpr int kUnit = kFp8 ? 16 : 8;       // elements in 16 bytes
     constexpr int kStep = 32 / Cfg::kChunks;   // rows per copy of the warp
+    constexpr int kCopies = kTok / kStep;
     uint64_t mask = 0;
 #pragma unroll
     for (int i = 0; i < kIds; ++i) {
@@ -360,7 +379,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
     const uint32_t at = stage * Cfg::kStage;
     if (mask == kFull) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kCopies; ++i) {
         const uint2 x = off[i * kStep];
         cp_async16(k_dst + at + i * kStep * kRowK, k_base + static_cast<uint64_t>(x.x) * 16);
         cp_async16(v_dst + at + i * kStep * kRowV, v_base + static_cast<uint64_t>(x.y) * 16);
@@ -368,7 +387,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
     } else if (mask) {
       // rows that do not count are filled with zeros
 #pragma unroll 1
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kCopies; ++i) {
         const uint2 x = off[i * kStep];
         const uint32_t n = (mask >> (lane / Cfg::kChunks + i * kStep)) & 1 ? 16 : 0;
         cp_async16_or_zero(k_dst + at + i * kStep * kRowK, k_base + static_cast<uint64_t>(x.x) * 16, n);
@@ -686,14 +705,13 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
       }
     }
     if (!whole) {
-      __threadfence();
-      __syncthreads();
+      // (the barrier at the end of the loop above puts the CTA's stores before
+      // this release, and the one below puts its acquire before their loads)
       if (tid == 0) s_last = atomic_add_acq_rel_gpu(p.counters + first, 1) == last - first;
       __syncthreads();
       if (s_last) {
         // join the ranges' partial results in range order: a warp per head, its
         // lanes over the head's values
-        __threadfence();
         if (tid == 0) p.counters[first] = 0;
         const int n = last - first + 1;
         auto part = [&](int i) {
@@ -704,25 +722,12 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
           constexpr int kPer = D / 32;           // values per lane
           float v[kPer] = {}, mm = -INFINITY, ll = 0.0f;
           for (int i0 = 0; i0 < n; i0 += 32) {
-            // lane i: range i0 + i
+            // lane i: range i0 + i; the first results on their way with the weights
             const int k = min(32, n - i0);
             const float mi = lane < k ? __ldcg(part(i0 + lane) + 8 * kNT * D + h) : -INFINITY;
             const float li = lane < k ? __ldcg(part(i0 + lane) + 8 * kNT * (D + 1) + h) : 0.0f;
-            float mx = mi;
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            mx = fmaxf(mx, mm);
-            const float old = mm == -INFINITY ? 0.0f : ex2(mm - mx);
-            const float a = mi == -INFINITY ? 0.0f : ex2(mi - mx);
-            float sum = a * li;
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            ll = ll * old + sum;
-            mm = mx;
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) v[e] *= old;
-            for (int i = 0; i < k; i += kAhead) {
-              float x[kAhead][kPer];
+            float x[kAhead][kPer];
+            auto fetch = [&](int i) {
 #pragma unroll
               for (int u = 0; u < kAhead; ++u)
                 if (i + u < k) {
@@ -739,6 +744,23 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Deco
                     x[u][1] = y.y;
                   }
                 }
+            };
+            fetch(0);
+            float mx = mi;
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
+            mx = fmaxf(mx, mm);
+            const float old = mm == -INFINITY ? 0.0f : ex2(mm - mx);
+            const float a = mi == -INFINITY ? 0.0f : ex2(mi - mx);
+            float sum = a * li;
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
+            ll = ll * old + sum;
+            mm = mx;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[e] *= old;
+            for (int i = 0; i < k; i += kAhead) {
+              if (i > 0) fetch(i);
 #pragma unroll
               for (int u = 0; u < kAhead; ++u) {
                 const float f = __shfl_sync(0xffffffffu, a, (i + u) & 31);

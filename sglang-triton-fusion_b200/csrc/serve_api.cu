@@ -119,8 +119,7 @@ int logprobs_cluster(int T, int V, int sm_count) {
 }
 
 // ----------------------------------------------------------------- decode --
-constexpr int kDecCtasPerSm = 2;
-static_assert(kDecCounterBytes / 4 >= 1024, "a counter per CTA");
+constexpr int kDecCtasPerSm = 4;      // at most
 
 size_t decode_workspace_bytes(int group, int D, int sm_count) {
   return kDecCounterBytes +
@@ -129,13 +128,14 @@ size_t decode_workspace_bytes(int group, int D, int sm_count) {
 
 template <int D, bool kFp8, int kNT>
 cudaError_t launch_decode(const DecodeParams& p, const DeviceInfo& di, fp8gq_stream_t stream) {
-  using Cfg = DecCfg<D, kFp8>;
+  using Cfg = DecCfg<D, kFp8, kNT>;
   auto fn = paged_decode_kernel<D, kFp8, kNT>;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(fn), static_cast<int>(Cfg::kSmem));
   if (e != cudaSuccess) return e;
   // no more CTAs than tiles, were every sequence as long as its page table
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.cache.page_size + Cfg::kTile - 1) / Cfg::kTile;
-  int64_t grid = kDecCtasPerSm * di.sm_count;
+  int64_t grid = Cfg::kCtas * di.sm_count;
+  if (grid * 4 > kDecCounterBytes) grid = kDecCounterBytes / 4;      // a counter per CTA
   const int64_t most = tiles > grid ? grid : tiles * p.Hkv * p.blocks * p.B;
   if (most < grid) grid = most < 1 ? 1 : most;
   return launch_with_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(kDecThreads), Cfg::kSmem,
