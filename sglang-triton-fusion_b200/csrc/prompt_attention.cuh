@@ -27,6 +27,12 @@
 // written.  (A CTA per item spent 13000 cycles of its own before and after its
 // tiles: as much as 6 tiles take.)
 //
+// Few items over long keys are cut instead: the key tiles of all items, in one
+// list, go to the CTAs in equal ranges.  An item that lies in one range is
+// written as above; of one that lies in several, each CTA leaves its piece (O as
+// it is and the rows' m and l, fp32) in the workspace, and prompt_join_kernel
+// adds them in the order of the keys, rescaled to the largest m.
+//
 // The two tiles' warps that share a scheduler take turns at the exponentials:
 // left alone they fall into step, both in the MUFU at half speed and then both
 // waiting (1 x 8192: 453 against 526 us).  Computing a part of them on the fma
@@ -44,6 +50,13 @@
 
 namespace fp8gq {
 
+// An item whose keys several CTAs share: CTA c of its first piece to `last`.
+struct PrSplit {
+  int q0, lq, r0, hk;
+  int last;                 // -1: none begins in CTA c
+  int pad[3];
+};
+
 struct PromptParams {
   __nv_bfloat16* out;
   float* lse;
@@ -57,6 +70,9 @@ struct PromptParams {
   float scale_log2;         // |scale| log2(e)
   int negate;               // scale < 0
   int causal;
+  int split;                // equal ranges of key tiles instead of whole items
+  PrSplit* splits;          // [grid]
+  float* parts;             // [grid][2][PrCfg::kPart]: the piece that a CTA's range begins, ends with
 };
 
 constexpr int kPrThreads = 384;
@@ -74,6 +90,8 @@ struct PrCfg {
   // TMEM columns: O0 O1 S0 S1 P0 P1
   static constexpr int kS = 2 * D, kP = kS + 2 * kKeys, kPCols = (kKeys / 2 + 15) / 16 * 16;
   static_assert(kP + 2 * kPCols <= 512, "TMEM");
+  // a piece's result: [2 query tiles][D / 4][128 rows][4] O, then [2][128] (m, l)
+  static constexpr int kPartO = 2 * 128 * D, kPart = kPartO + 2 * 128 * 2;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -169,8 +187,16 @@ struct PrWork {
   int r0;                   // first token of the item within the sequence
   int hk;
   int n[2];                 // key tiles that the last row of each query tile sees
+  int part;                 // >= 0: a piece, whose result goes there
 };
-constexpr int kPrItems = 2; // items looked up ahead
+constexpr int kPrItems = 2;      // items looked up ahead
+// What an item's start and end count in its range, in key tiles (4 x 1024 ragged
+// behind 5003, D = 64, and 1 x 4096, 2 kv heads: 2: 59 and 51 us, 4: 61 and 49,
+// 8: 64 and 52), and the least range (4 x 16 behind 4000: 6: 25 us, 10: 28, 16:
+// 35; above kPrItemCost, so that no range is an item's start alone).
+constexpr int kPrItemCost = 4;
+constexpr int kPrMinTiles = 6;
+static_assert(kPrMinTiles > kPrItemCost, "");
 
 template <int D>
 __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const __grid_constant__ CUtensorMap tq,
@@ -264,6 +290,33 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
           q1 = min(max(q1, q0), p.Tq);
         }
       };
+      auto keys = [&](int b, int& k0, int& k1) {
+        k0 = __ldg(p.cu_k + b);
+        k1 = __ldg(p.cu_k + b + 1);
+        if (k0 < 0 || k0 > p.Tk || k1 < k0 || k1 > p.Tk) {
+          record_error(kSiteBadIndex);
+          k0 = min(max(k0, 0), p.Tk);
+          k1 = min(max(k1, k0), p.Tk);
+        }
+      };
+      // key tiles that the query tiles of the item at token r0 see
+      auto seen_tiles = [&](int r0, int lq, int lk, int* n) {
+        for (int i = 0; i < 2; ++i) {
+          const int end = min(r0 + (i + 1) * p.rows, lq);          // past the query tile's last token
+          int seen = end > r0 + i * p.rows ? lk : 0;
+          if (p.causal && seen) seen = min(lk, max(0, end + lk - lq));
+          n[i] = (seen + kKeys - 1) / kKeys;
+        }
+      };
+      int it = 0;
+      auto post = [&](const PrWork& x, bool writer) {              // the next item, or the end
+        if (it >= kPrItems) ok = pr_wait_warp(&b_taken[it % kPrItems], (it / kPrItems - 1) & 1);
+        if (!ok) return;
+        if (writer) s_work[it % kPrItems] = x;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_item[it % kPrItems]);
+        ++it;
+      };
       int mine = 0;
       for (int b = b_lo; b < b_hi; ++b) {
         int q0, q1;
@@ -276,58 +329,124 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         const int x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += x;
       }
-      const int total = __shfl_sync(0xffffffffu, incl, 31) * p.Hkv;
-      int id = blockIdx.x;                          // the first item; the others off the counter
-      for (int it = 0;; ++it) {
-        PrWork x;
-        x.q0 = -1;
-        const int tile = id / p.Hkv;
-        const bool here = id < total && tile < incl && tile >= incl - mine;
-        if (here) {
-          int at = incl - mine;
-          for (int b = b_lo; b < b_hi; ++b) {
-            int q0, q1;
-            tokens(b, q0, q1, false);
-            const int nb = (q1 - q0 + span - 1) / span;
-            if (tile < at + nb) {
-              int k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
-              if (k0 < 0 || k0 > p.Tk || k1 < k0 || k1 > p.Tk) {
-                record_error(kSiteBadIndex);
-                k0 = min(max(k0, 0), p.Tk);
-                k1 = min(max(k1, k0), p.Tk);
+      const int tiles = __shfl_sync(0xffffffffu, incl, 31), total = tiles * p.Hkv;
+      PrWork x;
+      x.q0 = -1;
+      x.part = -1;
+      if (p.split) {
+        // ---- equal ranges: lane b has sequence b ----
+        int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+        if (lane < p.B) {
+          tokens(lane, q0, q1, false);
+          keys(lane, k0, k1);
+        }
+        const int lq = q1 - q0, lk = k1 - k0;
+        // this lane's tile of the 32 from `from` on; what an item of it counts
+        int yb, ynb, yn[2];
+        auto look = [&](int from) {
+          const int t = from + lane;
+          yb = 0;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) yb += __shfl_sync(0xffffffffu, incl, yb + o - 1) <= t ? o : 0;
+          const int at = __shfl_sync(0xffffffffu, incl - mine, yb), nb = __shfl_sync(0xffffffffu, mine, yb);
+          const int ylq = __shfl_sync(0xffffffffu, lq, yb), ylk = __shfl_sync(0xffffffffu, lk, yb);
+          ynb = (nb - 1 - (t - at)) * span;                        // its first token
+          if (t >= tiles) return 0;
+          seen_tiles(ynb, ylq, ylk, yn);
+          return max(yn[0], yn[1]) + kPrItemCost;
+        };
+        int64_t work = 0;
+        for (int from = 0; from < tiles; from += 32) work += __reduce_add_sync(0xffffffffu, static_cast<unsigned>(look(from)));
+        work *= p.Hkv;
+        const int64_t ctas = max(min(static_cast<int64_t>(gridDim.x), work / kPrMinTiles), static_cast<int64_t>(1));
+        const int cta = static_cast<int>(blockIdx.x);
+        const int64_t lo = cta < ctas ? work * cta / ctas : work, hi = cta < ctas ? work * (cta + 1) / ctas : work;
+        PrSplit mark{};
+        mark.last = -1;
+        int64_t at = 0;
+        for (int from = 0; from < tiles && at < hi && ok; from += 32) {
+          const int cost = look(from);
+          int sum = cost;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+          }
+          const int64_t a0 = at + static_cast<int64_t>(sum - cost) * p.Hkv, a1 = at + static_cast<int64_t>(sum) * p.Hkv;
+          at = __shfl_sync(0xffffffffu, a1, 31);
+          uint32_t in = __ballot_sync(0xffffffffu, cost > 0 && a0 < hi && a1 > lo);
+          for (; in && ok; in &= in - 1) {
+            const int from_lane = __ffs(in) - 1;
+            const int64_t a = __shfl_sync(0xffffffffu, a0, from_lane);
+            const int c = __shfl_sync(0xffffffffu, cost, from_lane), n = c - kPrItemCost;
+            const int b = __shfl_sync(0xffffffffu, yb, from_lane), r0 = __shfl_sync(0xffffffffu, ynb, from_lane);
+            const int n0 = __shfl_sync(0xffffffffu, yn[0], from_lane), n1 = __shfl_sync(0xffffffffu, yn[1], from_lane);
+            const int xq0 = __shfl_sync(0xffffffffu, q0, b), xlq = __shfl_sync(0xffffffffu, lq, b);
+            const int xk0 = __shfl_sync(0xffffffffu, k0, b), xlk = __shfl_sync(0xffffffffu, lk, b);
+            for (int hk = lo > a ? static_cast<int>((lo - a) / c) : 0; hk < p.Hkv && a + static_cast<int64_t>(hk) * c < hi && ok; ++hk) {
+              const int64_t first = a + static_cast<int64_t>(hk) * c + kPrItemCost;      // its first key tile
+              const int j0 = static_cast<int>(min(max(lo - first, static_cast<int64_t>(0)), static_cast<int64_t>(n)));
+              const int j1 = static_cast<int>(min(max(hi - first, static_cast<int64_t>(0)), static_cast<int64_t>(n)));
+              // an item without keys belongs to the range that it begins in
+              if (j0 == j1 && (n > 0 || first - kPrItemCost < lo)) continue;
+              x.q0 = xq0;
+              x.lq = xlq;
+              x.k0 = xk0 + j0 * kKeys;
+              x.lk = xlk - j0 * kKeys;
+              x.r0 = r0;
+              x.hk = hk;
+              x.n[0] = max(min(n0, j1) - j0, 0);
+              x.n[1] = max(min(n1, j1) - j0, 0);
+              x.part = j1 - j0 == n ? -1 : 2 * cta + (j0 == 0 ? 1 : 0);
+              if (x.part >= 0 && j0 == 0) {
+                mark = PrSplit{xq0, xlq, r0, hk, static_cast<int>(((first + n) * ctas - 1) / work), {}};
               }
-              x.q0 = q0;
-              x.lq = q1 - q0;
-              x.k0 = k0;
-              x.lk = k1 - k0;
-              x.hk = id - tile * p.Hkv;
-              x.r0 = (nb - 1 - (tile - at)) * span;
-              for (int i = 0; i < 2; ++i) {
-                const int end = min(x.r0 + (i + 1) * p.rows, x.lq);      // past the query tile's last token
-                int seen = end > x.r0 + i * p.rows ? x.lk : 0;
-                if (p.causal && seen) seen = min(x.lk, max(0, end + x.lk - x.lq));
-                x.n[i] = (seen + kKeys - 1) / kKeys;
-              }
-              break;
+              post(x, lane == 0);
             }
-            at += nb;
           }
         }
-        if (it >= kPrItems) ok = pr_wait_warp(&b_taken[it % kPrItems], (it / kPrItems - 1) & 1);
-        if (!ok) break;
-        if (here || (lane == 0 && id >= total)) s_work[it % kPrItems] = x;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b_item[it % kPrItems]);
-        if (id >= total) break;
-        // not before this item's loads are issued: an item taken early is one that
-        // an idle CTA cannot take
-        ok = pr_wait_warp(&b_want, it & 1);
-        if (!ok) break;
-        if (lane == 0) id = gridDim.x + atomicAdd(p.counters, 1);
-        id = __shfl_sync(0xffffffffu, id, 0);
+        if (lane == 0) p.splits[cta] = mark;
+        x.q0 = -1;
+        if (ok) post(x, lane == 0);
+      } else {
+        int id = blockIdx.x;                          // the first item; the others off the counter
+        for (;;) {
+          x.q0 = -1;
+          const int tile = id / p.Hkv;
+          const bool here = id < total && tile < incl && tile >= incl - mine;
+          if (here) {
+            int at = incl - mine;
+            for (int b = b_lo; b < b_hi; ++b) {
+              int q0, q1;
+              tokens(b, q0, q1, false);
+              const int nb = (q1 - q0 + span - 1) / span;
+              if (tile < at + nb) {
+                int k0, k1;
+                keys(b, k0, k1);
+                x.q0 = q0;
+                x.lq = q1 - q0;
+                x.k0 = k0;
+                x.lk = k1 - k0;
+                x.hk = id - tile * p.Hkv;
+                x.r0 = (nb - 1 - (tile - at)) * span;
+                seen_tiles(x.r0, x.lq, x.lk, x.n);
+                break;
+              }
+              at += nb;
+            }
+          }
+          post(x, here || (lane == 0 && id >= total));
+          if (!ok || id >= total) break;
+          // not before this item's loads are issued: an item taken early is one that
+          // an idle CTA cannot take
+          ok = pr_wait_warp(&b_want, (it - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) id = gridDim.x + atomicAdd(p.counters, 1);
+          id = __shfl_sync(0xffffffffu, id, 0);
+        }
       }
       // the last CTA to get here leaves the counters as it found them
-      if (lane == 0) {
+      if (lane == 0 && !p.split) {
         __threadfence();
         if (atomicAdd(p.counters + 1, 1) == static_cast<int>(gridDim.x) - 1) {
           p.counters[0] = 0;
@@ -581,6 +700,30 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         if (!ok) break;
         tc_fence_after();
       }
+      if (w.part >= 0) {
+        // a piece: O as it is, and its (m, l), of the rows that there are
+        float* part = p.parts + static_cast<int64_t>(w.part) * Cfg::kPart;
+        if (mine > 0) {
+#pragma unroll 1
+          for (int x = 0; x < D; x += 16) {
+            uint32_t o[16];
+            tmem_ld16r(to + x, o);
+            tmem_wait_ld();
+            tmem_loaded16(o);
+            if (!live) continue;
+#pragma unroll
+            for (int y = 0; y < 16; y += 4)
+              *reinterpret_cast<uint4*>(part + ((i * (D / 4) + (x + y) / 4) * 128 + row) * 4) =
+                  make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b_out[i]);
+        }
+        if (live) *reinterpret_cast<float2*>(part + Cfg::kPartO + (i * 128 + row) * 2) = make_float2(m, l);
+        leave_item();
+        continue;
+      }
       const float r = l > 0.0f ? 1.0f / l : l;             // a row that sees nothing: 0; NaN stays
       // 64 values of each row at a time through shared memory (chunks swizzled
       // by row), so that the warp writes whole rows
@@ -640,6 +783,69 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
   if (warp == 9) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+  grid_launch_dependents();
+}
+
+// Joins the pieces of the items that several CTAs share, in the order of the
+// keys.  Block (c, x): the item that begins in CTA c and goes on, values 16 x to
+// 16 x + 15; warp: 32 rows, one per lane.
+template <int D>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p) {
+  using Cfg = PrCfg<D>;
+  grid_dependency_wait();
+  const int c = blockIdx.x, d0 = 16 * blockIdx.y;
+  const PrSplit e = p.splits[c];
+  if (e.last > c) {
+    const int i = threadIdx.x >> 7, row = threadIdx.x & 127;
+    const int row_tok = (row * p.group_inv) >> 16, row_head = row - row_tok * p.group;
+    const int tok = e.r0 + i * p.rows + row_tok;
+    if (row_tok < p.rows && tok < e.lq) {
+      const float* ml = p.parts + Cfg::kPartO + (i * 128 + row) * 2;
+      const float* po = p.parts + ((i * (D / 4) + d0 / 4) * 128 + row) * 4;
+      auto slot = [&](int k) { return static_cast<int64_t>(2 * k + (k == c ? 1 : 0)) * Cfg::kPart; };
+      float m = -INFINITY;
+#pragma unroll 4
+      for (int k = c; k <= e.last; ++k) m = fmaxf(m, ml[slot(k)]);
+      float l = 0.0f, acc[16];
+#pragma unroll
+      for (int y = 0; y < 16; ++y) acc[y] = 0.0f;
+#pragma unroll 2
+      for (int k = c; k <= e.last; ++k) {
+        const float2 r = *reinterpret_cast<const float2*>(ml + slot(k));
+        float4 o[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) o[y] = *reinterpret_cast<const float4*>(po + slot(k) + y * 512);
+        // a row that saw nothing there left no O; NaN stays
+        const bool none = r.x == -INFINITY && r.y == 0.0f;
+        const float a = r.x == -INFINITY ? 1.0f : ex2f((r.x - m) * p.scale_log2);
+        if (!none) {
+          l = fmaf(r.y, a, l);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            acc[4 * y] = fmaf(o[y].x, a, acc[4 * y]);
+            acc[4 * y + 1] = fmaf(o[y].y, a, acc[4 * y + 1]);
+            acc[4 * y + 2] = fmaf(o[y].z, a, acc[4 * y + 2]);
+            acc[4 * y + 3] = fmaf(o[y].w, a, acc[4 * y + 3]);
+          }
+        }
+      }
+      const float r = l > 0.0f ? 1.0f / l : l;
+      uint32_t h[8];
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(l == 0.0f ? 0.0f : acc[2 * y] * r, l == 0.0f ? 0.0f : acc[2 * y + 1] * r);
+        h[y] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      const int64_t t = static_cast<int64_t>(e.q0) + tok;
+      const int head = e.hk * p.group + row_head;
+      uint4* out = reinterpret_cast<uint4*>(p.out + t * p.o_token + head * p.o_head + d0);
+      out[0] = make_uint4(h[0], h[1], h[2], h[3]);
+      out[1] = make_uint4(h[4], h[5], h[6], h[7]);
+      if (d0 == 0 && p.lse)
+        p.lse[t * p.Hq + head] =
+            l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * p.scale_log2) + log2f(l)) * 0.6931471805599453f;
+    }
   }
   grid_launch_dependents();
 }

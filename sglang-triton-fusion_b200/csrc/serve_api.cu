@@ -87,7 +87,31 @@ int check_rows(const void* p, int64_t token, int64_t head, int tokens, int heads
 }
 
 // ----------------------------------------------------------------- prompt --
-constexpr size_t kPromptWorkspaceBytes = 16;
+constexpr int kPromptSplitSeqs = 32;         // (a lane of the item warp has a sequence)
+constexpr int kPromptSplitGain = 1000;       // keys whose tiles take as long as pieces and their join cost
+
+// Whole items off a counter, or equal ranges of key tiles whose pieces are
+// joined: by the tiles that the busiest CTA computes when items are whole,
+// against the mean, for sequences of the mean lengths.  Measured, whole items and
+// ranges: 64 tokens behind 6000 (16 heads, 1 kv head) 93 and 25 us, 4 x 16 behind
+// 4000 (32, 8, D = 64) 54 and 25, 4 x 1024 ragged behind 5003 (16, 4, D = 64) 90
+// and 61, 2 x 700 behind 1000 (8, 8) 33 and 24; 1 x 2048 (32, 8) 42 and 54, 8 x 1
+// behind 700 15.5 and 18.5, 4 x 500 (40, 8) 30 and 37.
+bool prompt_split(int B, int Tq, int Tk, int Hkv, int span, int keys, bool causal, int sms) {
+  if (B > kPromptSplitSeqs) return false;
+  const int lq = (Tq + B - 1) / B;
+  const double most = static_cast<double>(Tk) / B / keys, own = std::min(causal ? static_cast<double>(lq) / keys : 0.0, most);
+  const double least = most - own;             // tiles of a sequence's last and of its first item
+  const double share = static_cast<double>(B) * ((lq + span - 1) / span) * Hkv / sms;
+  const double mean = share * (most - own / 2);
+  const double busiest = std::max(most, mean + (std::ceil(share) - share) * least);
+  return (busiest - mean) * keys >= kPromptSplitGain;
+}
+
+size_t prompt_workspace_bytes(int sm_count) {
+  return kDecCounterBytes + sm_count * (sizeof(PrSplit) + 2 * sizeof(float) * PrCfg<128>::kPart);
+}
+
 
 // [tokens, heads, D] bf16 as boxes of 64 values x `box_heads` heads x
 // `box_tokens` tokens, 128-byte swizzle.  A stride that no coordinate above 0
@@ -266,7 +290,11 @@ int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t 
   return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_paged_decode_attention");
 }
 
-size_t fp8gq_prompt_workspace_bytes(void) { return kPromptWorkspaceBytes; }
+size_t fp8gq_prompt_workspace_bytes(void) {
+  DeviceInfo di;
+  if (device_info(&di, nullptr) != FP8GQ_OK) return 0;
+  return prompt_workspace_bytes(di.sm_count);
+}
 
 int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                            int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
@@ -315,18 +343,23 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
       !make_heads_tmap(&tv, Tk ? v : q, Tk ? Tk : 1, Hkv, D, Tk ? v_token_stride : 0, Tk ? v_head_stride : D, 1, keys))
     return FP8GQ_ERR_LAUNCH;
   // a row block more than the tokens fill for each sequence's odd end
-  int64_t blocks = (static_cast<int64_t>(Tq) / (2 * p.rows) + B) * Hkv;
-  if (blocks > INT32_MAX / 2) return FP8GQ_ERR_UNSUPPORTED;
-  if (blocks > di.sm_count) blocks = di.sm_count;
-  if (!workspace || workspace_bytes < kPromptWorkspaceBytes) return FP8GQ_ERR_WORKSPACE;
+  const int64_t items = (static_cast<int64_t>(Tq) / (2 * p.rows) + B) * Hkv;
+  if (items > INT32_MAX / 2) return FP8GQ_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < prompt_workspace_bytes(di.sm_count)) return FP8GQ_ERR_WORKSPACE;
   if (!aligned16(workspace)) return FP8GQ_ERR_ALIGNMENT;
   p.counters = static_cast<int*>(workspace);
+  p.splits = reinterpret_cast<PrSplit*>(static_cast<char*>(workspace) + kDecCounterBytes);
+  p.parts = reinterpret_cast<float*>(p.splits + di.sm_count);
+  p.split = prompt_split(B, Tq, Tk, Hkv, 2 * p.rows, keys, causal != 0, di.sm_count);
+  const unsigned blocks = static_cast<unsigned>(p.split || items > di.sm_count ? di.sm_count : items);
   auto fn = D == 128 ? prompt_attention_kernel<128> : prompt_attention_kernel<64>;
   const size_t smem = D == 128 ? PrCfg<128>::kSmem : PrCfg<64>::kSmem;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(fn), static_cast<int>(smem));
   if (e == cudaSuccess)
-    e = launch_with_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(kPrThreads), smem,
-                        static_cast<cudaStream_t>(stream), tq, tk, tv, p);
+    e = launch_with_pdl(fn, dim3(blocks), dim3(kPrThreads), smem, static_cast<cudaStream_t>(stream), tq, tk, tv, p);
+  if (e == cudaSuccess && p.split)
+    e = launch_with_pdl(D == 128 ? prompt_join_kernel<128> : prompt_join_kernel<64>, dim3(blocks, D / 16), dim3(256), 0,
+                        static_cast<cudaStream_t>(stream), p);
   return e == cudaSuccess ? launch_status() : cuda_fail(e, "fp8gq_prompt_attention");
 }
 

@@ -36,6 +36,7 @@ def _stream(device) -> int:
 
 
 _workspaces: dict = {}
+_outgrown: list = []    # scratch that a captured graph may still use
 _ws_bytes: dict = {}
 
 
@@ -65,6 +66,8 @@ def _workspace_entry(device: torch.device, nbytes: int, stream: int):
     key = (device.index, stream)
     ent = _workspaces.get(key)
     if ent is None or ent[2] < nbytes:
+        if ent is not None:
+            _outgrown.append(ent[0])
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         ent = (buf, buf.data_ptr(), buf.numel())
         _workspaces[key] = ent

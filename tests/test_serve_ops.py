@@ -432,6 +432,43 @@ def test_prompt_sharp_scores_strides_and_streams(f):
     check_prompt(f, q, k, v, cu, None)
 
 
+@pytest.mark.parametrize("lq,lk,hq,hkv,d", [
+    ([1], [6000], 8, 2, 128), ([64], [5003], 16, 1, 128), ([1, 0, 33, 7], [4000, 900, 0, 3333], 8, 4, 64),
+    ([300, 20], [2000, 4001], 10, 2, 128), ([700], [1900], 4, 4, 128), ([1300, 1], [1300, 5000], 4, 1, 64),
+    ([130] * 3 + [5] * 29, [3000, 2999, 1] + [2000] * 29, 2, 1, 64), ([2], [3000], 128, 1, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_few_rows_over_long_keys(f, lq, lk, hq, hkv, d, causal):
+    """Items that several CTAs share."""
+    q, k, v, cu_q, cu_k = prompt_case(sum(lk), lq, lk, hq, hkv, d)
+    check_prompt(f, q, k, v, cu_q, cu_k, causal)
+
+
+def test_prompt_shared_items_repeat_and_take_other_values(f):
+    q, k, v, cu_q, cu_k = prompt_case(11, [40, 3], [3100, 2500], 8, 2, 128)
+    out, lse = check_prompt(f, q, k, v, cu_q, cu_k)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o, s = f.prompt_attention(q, k, v, cu_q, cu_k, return_lse=True)
+    for _ in range(3):
+        o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o[:43], out[:43]) and torch.equal(s[:43], lse[:43])
+    # sharp scores in one part of the keys, the lowest in another; other lengths in the same graph
+    k[100:140] *= 30
+    k[2000:2100] *= -30
+    cu_q.copy_(torch.tensor([0, 1, 43]))
+    cu_k.copy_(torch.tensor([0, 2400, 5600]))
+    g.replay()
+    want, wlse = check_prompt(f, q, k, v, cu_q, cu_k)
+    assert torch.equal(o[:43], want[:43]) and torch.equal(s[:43], wlse[:43])
+    # a NaN key reaches the rows that see it, in whichever piece it lies
+    k[50] = float("nan")
+    o2, _ = f.prompt_attention(q, k, v, cu_q, cu_k, return_lse=True)
+    assert torch.isnan(o2[0]).any() and torch.equal(o2[1:43], want[1:43])
+
+
 def test_prompt_empty_and_out_of_range(f):
     q, k, v, cu, _ = prompt_case(6, [40], [40], 4, 2, 64, spare=0)
     assert f.prompt_attention(q[:0], k[:0], v[:0], torch.zeros(1, dtype=torch.int32, device="cuda")).shape == (0, 4, 64)
