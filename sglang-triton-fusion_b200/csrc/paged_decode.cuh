@@ -86,8 +86,8 @@ struct DecCfg {
   static constexpr int kRowV = kRow + 16;
   static constexpr int kStage = kTok * (kRowK + kRowV);
   static constexpr int kPad = D + 4;                    // o in shared memory: conflict-free fragment writes
-  static constexpr size_t kSmem = static_cast<size_t>(kDecWarps) * kDecStages * kStage +
-                                  sizeof(float) * kDecWarps * 2 * kPad;
+  static_assert(kStage >= 8 * kNT * kPad * 4 && kStage % 16 == 0, "a warp's o fits in a stage");
+  static constexpr size_t kSmem = static_cast<size_t>(kDecWarps) * kDecStages * kStage;
 };
 
 // Floats of one partial result: o [8 NT][D], m [8 NT], l [8 NT].
@@ -211,12 +211,11 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<D, kFp8, kNT>::kCtas) page
   __shared__ int64_t s_wsum[kDecWarps];
   __shared__ uint2 s_off[kDecWarps][kTok];                // a step's rows of k and v, in 16 bytes from the cache's base
   __shared__ uint64_t s_mask[kDecWarps][kDecStages];      // a step's tokens that count
-  __shared__ float s_m[kDecWarps][2], s_l[kDecWarps][2];
+  __shared__ float s_m[kDecWarps][8 * kNT], s_l[kDecWarps][8 * kNT];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * (kDecStages * Cfg::kStage);
-  float* s_o = reinterpret_cast<float*>(smem + kDecWarps * kDecStages * Cfg::kStage);
   const int items = p.Hkv * p.blocks;
 
   grid_dependency_wait();
@@ -635,13 +634,17 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<D, kFp8, kNT>::kCtas) page
       }
     }
 
-    // ---- the item's result: the four warps joined, 2 heads at a time ----
+    // ---- the item's result: the four warps joined; each leaves its sums where
+    // the rows of its last step were ----
     const int first = owner(cur.start + kDecItemCost), last = owner(cur.start + kDecItemCost + cur.n - 1);
     const bool whole = first == last;
     const int b = cur.b;
     float* slot = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == first ? 1 : 0)) * kSlot;
     next_item(cur);
     if (!cur.done) fetch_q(cur);               // arrives meanwhile
+    const int used = stage == 0 ? kDecStages - 1 : stage - 1;
+    auto sums = [&](int w) { return reinterpret_cast<float*>(smem + (w * kDecStages + used) * Cfg::kStage); };
+    __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
@@ -649,63 +652,63 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<D, kFp8, kNT>::kCtas) page
         l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], x);
         l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], x);
       }
+      const int h = 8 * nt + 2 * t4;                       // heads h, h + 1
+      if (h < heads) {
+        float* so = sums(warp) + h * Cfg::kPad;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int h2 = 8 * nt + 2 * q;                     // heads h2, h2 + 1
-        if (h2 >= heads) break;
-        if (t4 == q) {
-          float* so = s_o + warp * 2 * Cfg::kPad;
-#pragma unroll
-          for (int i = 0; i < kMT; ++i) {
-            const int d0 = kFp8 ? g * (D / 8) + 2 * i : 16 * i + g;
-            const int d1 = kFp8 ? d0 + 1 : d0 + 8;
-            so[d0] = o[nt][i][0];
-            so[d1] = o[nt][i][2];
-            so[Cfg::kPad + d0] = o[nt][i][1];
-            so[Cfg::kPad + d1] = o[nt][i][3];
-          }
-          if (g == 0) {
-            s_m[warp][0] = m[nt][0];
-            s_m[warp][1] = m[nt][1];
-            s_l[warp][0] = l[nt][0];
-            s_l[warp][1] = l[nt][1];
-          }
-        }
-        __syncthreads();
-        for (int i = tid; i < 2 * (D / 4); i += kDecThreads) {
-          const int h = i / (D / 4), d = (i % (D / 4)) * 4;
-          if (h2 + h >= heads) break;
-          float mm = s_m[0][h];
-#pragma unroll
-          for (int w = 1; w < kDecWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
-          float ll = 0.0f;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-          for (int w = 0; w < kDecWarps; ++w) {
-            const float a = s_m[w][h] == -INFINITY ? 0.0f : ex2(s_m[w][h] - mm);
-            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 2 + h) * Cfg::kPad + d);
-            ll += a * s_l[w][h];
-            v.x += a * x.x;
-            v.y += a * x.y;
-            v.z += a * x.z;
-            v.w += a * x.w;
-          }
-          if (whole) {
-            const float o4[4] = {v.x, v.y, v.z, v.w};
-            dec_store<4>(p, b, h0 + h2 + h, d, o4, mm, ll);
+        for (int i = 0; i < kMT; ++i) {
+          if constexpr (kFp8) {
+            const int d = g * (D / 8) + 2 * i;
+            *reinterpret_cast<float2*>(so + d) = make_float2(o[nt][i][0], o[nt][i][2]);
+            *reinterpret_cast<float2*>(so + Cfg::kPad + d) = make_float2(o[nt][i][1], o[nt][i][3]);
           } else {
-            *reinterpret_cast<float4*>(slot + (h2 + h) * D + d) = v;
-            if (d == 0) {
-              slot[8 * kNT * D + h2 + h] = mm;
-              slot[8 * kNT * (D + 1) + h2 + h] = ll;
-            }
+            const int d = 16 * i + g;
+            so[d] = o[nt][i][0];
+            so[d + 8] = o[nt][i][2];
+            so[Cfg::kPad + d] = o[nt][i][1];
+            so[Cfg::kPad + d + 8] = o[nt][i][3];
           }
         }
-        __syncthreads();
+        if (g == 0) {
+          s_m[warp][h] = m[nt][0];
+          s_m[warp][h + 1] = m[nt][1];
+          s_l[warp][h] = l[nt][0];
+          s_l[warp][h + 1] = l[nt][1];
+        }
       }
     }
+    __syncthreads();
+    for (int i = tid; i < heads * (D / 4); i += kDecThreads) {
+      const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+      float mm = s_m[0][h];
+#pragma unroll
+      for (int w = 1; w < kDecWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
+      float ll = 0.0f;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        const float a = s_m[w][h] == -INFINITY ? 0.0f : ex2(s_m[w][h] - mm);
+        const float4 x = *reinterpret_cast<const float4*>(sums(w) + h * Cfg::kPad + d);
+        ll += a * s_l[w][h];
+        v.x += a * x.x;
+        v.y += a * x.y;
+        v.z += a * x.z;
+        v.w += a * x.w;
+      }
+      if (whole) {
+        const float o4[4] = {v.x, v.y, v.z, v.w};
+        dec_store<4>(p, b, h0 + h, d, o4, mm, ll);
+      } else {
+        *reinterpret_cast<float4*>(slot + h * D + d) = v;
+        if (d == 0) {
+          slot[8 * kNT * D + h] = mm;
+          slot[8 * kNT * (D + 1) + h] = ll;
+        }
+      }
+    }
+    __syncthreads();                           // the sums have been read
     if (!whole) {
-      // (the barrier at the end of the loop above puts the CTA's stores before
+      // (the barrier above puts the CTA's stores before
       // this release, and the one below puts its acquire before their loads)
       if (tid == 0) s_last = atomic_add_acq_rel_gpu(p.counters + first, 1) == last - first;
       __syncthreads();
@@ -717,60 +720,79 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<D, kFp8, kNT>::kCtas) page
         auto part = [&](int i) {
           return p.partials + (static_cast<int64_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * kSlot;
         };
-        for (int h = warp; h < heads; h += kDecWarps) {
-          constexpr int kAhead = 8;
-          constexpr int kPer = D / 32;           // values per lane
-          float v[kPer] = {}, mm = -INFINITY, ll = 0.0f;
+        constexpr int kAhead = 8;
+        constexpr int kPer = D / 32;             // values per lane
+        for (int h0w = warp; h0w < heads; h0w += 2 * kDecWarps) {
+          // two heads at a time, so that their loads run side by side
+          float v[2][kPer] = {}, mm[2] = {-INFINITY, -INFINITY}, ll[2] = {};
           for (int i0 = 0; i0 < n; i0 += 32) {
             // lane i: range i0 + i; the first results on their way with the weights
             const int k = min(32, n - i0);
-            const float mi = lane < k ? __ldcg(part(i0 + lane) + 8 * kNT * D + h) : -INFINITY;
-            const float li = lane < k ? __ldcg(part(i0 + lane) + 8 * kNT * (D + 1) + h) : 0.0f;
-            float x[kAhead][kPer];
+            float mi[2], li[2], x[2][kAhead][kPer];
             auto fetch = [&](int i) {
 #pragma unroll
-              for (int u = 0; u < kAhead; ++u)
-                if (i + u < k) {
-                  const float* src = part(i0 + i + u) + h * D + kPer * lane;
-                  if constexpr (kPer == 4) {
-                    const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
-                    x[u][0] = y.x;
-                    x[u][1] = y.y;
-                    x[u][2] = y.z;
-                    x[u][3] = y.w;
-                  } else {
-                    const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
-                    x[u][0] = y.x;
-                    x[u][1] = y.y;
+              for (int z = 0; z < 2; ++z) {
+                const int h = h0w + z * kDecWarps;
+                if (h >= heads) break;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                  if (i + u < k) {
+                    const float* src = part(i0 + i + u) + h * D + kPer * lane;
+                    if constexpr (kPer == 4) {
+                      const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+                      x[z][u][0] = y.x;
+                      x[z][u][1] = y.y;
+                      x[z][u][2] = y.z;
+                      x[z][u][3] = y.w;
+                    } else {
+                      const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+                      x[z][u][0] = y.x;
+                      x[z][u][1] = y.y;
+                    }
                   }
-                }
+              }
             };
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const int h = h0w + z * kDecWarps;
+              const bool ok = lane < k && h < heads;
+              mi[z] = ok ? __ldcg(part(i0 + lane) + 8 * kNT * D + h) : -INFINITY;
+              li[z] = ok ? __ldcg(part(i0 + lane) + 8 * kNT * (D + 1) + h) : 0.0f;
+            }
             fetch(0);
-            float mx = mi;
+            float a[2];
 #pragma unroll
-            for (int y = 16; y > 0; y >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
-            mx = fmaxf(mx, mm);
-            const float old = mm == -INFINITY ? 0.0f : ex2(mm - mx);
-            const float a = mi == -INFINITY ? 0.0f : ex2(mi - mx);
-            float sum = a * li;
+            for (int z = 0; z < 2; ++z) {
+              float mx = mi[z];
 #pragma unroll
-            for (int y = 16; y > 0; y >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
-            ll = ll * old + sum;
-            mm = mx;
+              for (int y = 16; y > 0; y >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
+              mx = fmaxf(mx, mm[z]);
+              const float old = mm[z] == -INFINITY ? 0.0f : ex2(mm[z] - mx);
+              a[z] = mi[z] == -INFINITY ? 0.0f : ex2(mi[z] - mx);
+              float sum = a[z] * li[z];
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) v[e] *= old;
+              for (int y = 16; y > 0; y >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
+              ll[z] = ll[z] * old + sum;
+              mm[z] = mx;
+#pragma unroll
+              for (int e = 0; e < kPer; ++e) v[z][e] *= old;
+            }
             for (int i = 0; i < k; i += kAhead) {
               if (i > 0) fetch(i);
 #pragma unroll
-              for (int u = 0; u < kAhead; ++u) {
-                const float f = __shfl_sync(0xffffffffu, a, (i + u) & 31);
-                if (i + u < k)
+              for (int z = 0; z < 2; ++z)
 #pragma unroll
-                  for (int e = 0; e < kPer; ++e) v[e] = __fmaf_rn(f, x[u][e], v[e]);
-              }
+                for (int u = 0; u < kAhead; ++u) {
+                  const float f = __shfl_sync(0xffffffffu, a[z], (i + u) & 31);
+                  if (i + u < k)
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) v[z][e] = __fmaf_rn(f, x[z][u][e], v[z][e]);
+                }
             }
           }
-          dec_store<kPer>(p, b, h0 + h, kPer * lane, v, mm, ll);
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+            if (h0w + z * kDecWarps < heads) dec_store<kPer>(p, b, h0 + h0w + z * kDecWarps, kPer * lane, v[z], mm[z], ll[z]);
         }
       }
     }
