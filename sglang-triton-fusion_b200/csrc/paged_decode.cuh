@@ -17,7 +17,7 @@
 // order, so the result does not depend on who is last.
 //
 // Inside a CTA each warp runs alone: its lanes look up the pages of its own
-// kTok tokens and copy their rows of k and v (4 or 8 KB per step, kDecStages steps in
+// kTok tokens and copy their rows of k and v (8 KB per step, kDecStages steps in
 // flight), and it computes on them with matrix instructions whose M side is the
 // tokens (S^T = K Q^T, 16 x 8) and then the head's values (O^T = V^T P^T), so a
 // group of up to 8 query heads wastes nothing of K and V and no barrier stands
@@ -60,6 +60,7 @@ struct DecodeParams {
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecStages = 3;
+constexpr int kDecCtas = 2;                 // per SM (of 4 KB steps, four: 128 x 2047 e4m3, D = 64, 36 us against 25)
 constexpr int kDecCounterBytes = 16384;     // the workspace's counters (the tile kernel's too)
 // Tiles per CTA below which fewer CTAs work (1 x 333 and 1 x 2000 tokens: 1: 8.2
 // and 11.3 us; 2: 8.6 and 9.5; 3: 9.7 and 10.6).
@@ -70,12 +71,7 @@ constexpr int kDecItemCost = 2;
 
 template <int D, bool kFp8, int kNT>
 struct DecCfg {
-  // Two CTAs per SM of 8 KB steps; at 64 e4m3 values a head, four of 4 KB (128 x
-  // 2047 tokens, 2 kv heads: 39 against 45 us; the other kinds are slower that
-  // way: 8 x 32768 e4m3 at D = 128 186 against 98 us, 128 ragged bf16 at D = 64
-  // 30 against 21 us).
-  static constexpr int kCtas = D == 64 && kFp8 && kNT == 1 ? 4 : 2;
-  static constexpr int kStep = kCtas == 4 ? 4096 : 8192;      // bytes of k and v rows of one warp's step
+  static constexpr int kStep = 8192;                    // bytes of k and v rows of one warp's step
   static constexpr int kRow = D * (kFp8 ? 1 : 2);       // bytes of a row
   static constexpr int kTok = kStep / 2 / kRow;
   static constexpr int kTile = kTok * kDecWarps;
@@ -200,7 +196,7 @@ struct DecWalk {
 };
 
 template <int D, bool kFp8, int kNT>
-__global__ void __launch_bounds__(kDecThreads, DecCfg<D, kFp8, kNT>::kCtas) paged_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(const DecodeParams p) {
   using Cfg = DecCfg<D, kFp8, kNT>;
   constexpr int kTok = Cfg::kTok, kTile = Cfg::kTile, kMT = D / 16, kKT = D / 16, kTT = kTok / 16;
   constexpr int kSlot = dec_slot_floats(D, kNT);

@@ -143,11 +143,10 @@ int logprobs_cluster(int T, int V, int sm_count) {
 }
 
 // ----------------------------------------------------------------- decode --
-constexpr int kDecCtasPerSm = 4;      // at most
 
 size_t decode_workspace_bytes(int group, int D, int sm_count) {
   return kDecCounterBytes +
-         static_cast<size_t>(kDecCtasPerSm) * sm_count * 2 * dec_slot_floats(D, group > 8 ? 2 : 1) * sizeof(float);
+         static_cast<size_t>(kDecCtas) * sm_count * 2 * dec_slot_floats(D, group > 8 ? 2 : 1) * sizeof(float);
 }
 
 template <int D, bool kFp8, int kNT>
@@ -158,7 +157,7 @@ cudaError_t launch_decode(const DecodeParams& p, const DeviceInfo& di, fp8gq_str
   if (e != cudaSuccess) return e;
   // no more CTAs than tiles, were every sequence as long as its page table
   const int64_t tiles = (static_cast<int64_t>(p.max_pages) * p.cache.page_size + Cfg::kTile - 1) / Cfg::kTile;
-  int64_t grid = Cfg::kCtas * di.sm_count;
+  int64_t grid = kDecCtas * di.sm_count;
   if (grid * 4 > kDecCounterBytes) grid = kDecCounterBytes / 4;      // a counter per CTA
   const int64_t most = tiles > grid ? grid : tiles * p.Hkv * p.blocks * p.B;
   if (most < grid) grid = most < 1 ? 1 : most;
