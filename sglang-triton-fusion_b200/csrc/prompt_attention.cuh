@@ -1,7 +1,7 @@
 // Attention over packed prompts on the 5th-generation tensor cores.
 //
-// Mathematics: per query row, one pass over the keys in tiles of 128 with the
-// running maximum m and sum l of the softmax; O is rescaled when m moves.
+// Mathematics: per query row, one pass over the keys in tiles of kKeys with the
+// running maximum m and sum l of the softmax; O is rescaled when m moves far.
 //
 // Bound: the tensor cores (4 D flops per visible pair and head) and, next to
 // them, the exponentials: those of a tile keep the MUFU as busy as its two
@@ -16,9 +16,11 @@
 // (bf16, the A operand of the second product straight from TMEM) and O.  P has
 // columns of its own, so that the next scores are computed while the softmax
 // works on these; that is what sets kKeys: 80 keys at D = 128 (S 80 + P 40 + O
-// 128 columns, twice, of 512), 128 at D = 64.  With 128 keys and P over S at
-// D = 128, the softmax waited 1900 of 4100 cycles a tile for the products and
-// 8192 tokens took 607 us.  v is read as it lies (its N side contiguous).
+// 128 columns, twice, of 512), 128 at D = 64.  (1 x 8192 at D = 128, 32 and 8
+// heads: 471 us; 128 keys with P over S, whose next products wait for the weights:
+// 536 to 569; 64 keys with P over two S in turn, where nothing waits but a product
+// takes as long for 64 columns as for 80: 535.)  v is read as it lies (its N side
+// contiguous).
 //
 // One CTA per SM takes items (two query tiles of one kv head) off a common
 // counter, the last rows of a sequence first.  Every role runs on into the next
@@ -38,6 +40,10 @@
 // waiting (1 x 8192: 453 against 526 us).  Computing a part of them on the fma
 // pipe instead (2^n times a polynomial) was slower at every part: the two warps
 // of a scheduler have no issue slots to spare.
+//
+// Measured, causal: 1 x 8192 (32 query and 8 kv heads of 128) 453 to 538 us from
+// one board to the next (1.0 to 1.2 PFLOP/s), 8 ragged to 700 38 us (fixed cost of
+// a call 7, of an item 2 to 4), 4 x 1024 ragged behind 5003 (16, 4, D = 64) 61 us.
 //
 // Warps 0-3 and 4-7: softmax, output (one thread per row of tile 0, 1).  Warp 8:
 // TMA; it also clears the rows of the last v tile that lie past the sequence
@@ -212,6 +218,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
   __shared__ uint64_t b_full[kSlots], b_free[kSlots];
   __shared__ uint64_t b_s[2], b_r[2], b_p[2], b_o[2];        // scores ready, read; weights ready; O updated
   __shared__ uint64_t b_out[2];                              // O read
+  __shared__ uint64_t b_end[2];                              // after a wait gave up: the products issued are done
   __shared__ uint64_t b_turn[2][4];                          // tile i's warp may have the MUFU
   __shared__ uint32_t s_tmem;
   __shared__ PrWork s_work[kPrItems];
@@ -243,6 +250,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         mbar_init(&b_p[i], 4);
         mbar_init(&b_o[i], 1);
         mbar_init(&b_out[i], 4);
+        mbar_init(&b_end[i], 1);
         for (int x = 0; x < 4; ++x) mbar_init(&b_turn[i][x], 1);
       }
       fence_mbar_init();
@@ -456,12 +464,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
     } else if (warp == 8) {
       // ---- TMA ----
       int x0 = 0, items = 0, tails = 0;             // k and v tiles, items and tails so far
+      int q_sent = 0, sent = 0;                     // q, k and v tiles on their way or there
       while (next_item()) {
         const int n = max(w.n[0], w.n[1]);
         const bool partial = n * kKeys > w.lk;      // the last tile reaches past the sequence
         if (n > 0) {
           if (items > 0) ok = pr_wait_warp(&b_qfree, (items - 1) & 1);
           if (!ok) break;
+          ++q_sent;
           if (pr_elect()) {
             mbar_arrive_expect_tx(&b_q, 2 * Cfg::kHalves * p.group * p.rows * 128);
             for (int i = 0; i < 2; ++i)
@@ -473,6 +483,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             const int x = x0 + i, slot = x % kSlots;
             if (x >= kSlots) ok = pr_wait_warp(&b_free[slot], (x / kSlots - 1) & 1);
             if (!ok) break;
+            ++sent;
             if (pr_elect()) {
               uint64_t* bar = partial && i == 2 * n - 1 ? &b_tail : &b_full[slot];
               mbar_arrive_expect_tx(bar, kTile);
@@ -506,8 +517,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       // the copies that no one has waited for have landed before the CTA ends
       // (only after a wait gave up: otherwise every tile has been used)
       if (!ok && lane == 0) {
-        pr_wait(&b_q, items & 1);
-        for (int i = 0; i < kSlots; ++i) pr_wait(&b_full[i], (x0 / kSlots) & 1);
+        if (q_sent) pr_wait(&b_q, (q_sent - 1) & 1);
+        for (int x = max(sent - kSlots, 0); x < sent; ++x) pr_wait(&b_full[x % kSlots], (x / kSlots) & 1);
       }
     } else {
       // ---- MMA of tile i: the warp waits together, one lane issues ----
@@ -574,9 +585,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         leave_item();
       }
       if (!ok) {                                           // what has been issued completes
-        if (pr_elect()) mma_commit(&b_o[i]);
+        if (pr_elect()) mma_commit(&b_end[i]);
         __syncwarp();
-        pr_wait_warp(&b_o[i], step0 & 1);
+        pr_wait_warp(&b_end[i], 0);
       }
     }
   } else {
