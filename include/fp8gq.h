@@ -600,7 +600,8 @@ int fp8gq_qk_norm_rope_append(const void *qkv, int64_t ldqkv, const int64_t *pos
  * word.  Slots past a sequence's length may hold anything, NaN included.
  * workspace as for the tile kernel: fp8gq_paged_decode_workspace_bytes bytes,
  * zero-filled before its first use; may be shared with the tile kernel's
- * calls of the same stream.  D is 64 or 128; Hq is a multiple of Hkv. */
+ * calls of the same stream.  D is 64 or 128; Hq is a multiple of Hkv.  The
+ * cache's k, and its v, span at most 64 GB. */
 size_t fp8gq_paged_decode_workspace_bytes(int Hq, int Hkv, int D);
 int fp8gq_paged_decode_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
                                  const fp8gq_paged_cache *cache, const int32_t *page_table,
@@ -622,7 +623,8 @@ int fp8gq_paged_decode_attention(const void *q, int64_t q_token_stride, int64_t 
  * sequence's own k and v are taken to be finite (a masked v that is infinite
  * or NaN may reach the rows of its tile).  An offset out of range is cut to
  * [0, Tq] or [0, Tk] and recorded in the device error word.
- * workspace: fp8gq_prompt_workspace_bytes bytes, as for fp8gq_paged_decode_attention.
+ * workspace: fp8gq_prompt_workspace_bytes bytes (0 without a usable device), as
+ * for fp8gq_paged_decode_attention.
  * At most 128 query heads per kv head; scale is finite. */
 size_t fp8gq_prompt_workspace_bytes(void);
 int fp8gq_prompt_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,

@@ -26,8 +26,8 @@
 // 235 us against 131 as the rest stood then).
 //
 // Measured, 32 query and 8 kv heads of 128: 64 x 4096 tokens 179 us (6.0 TB/s),
-// 48 ragged to 6000 72 us (5.5 TB/s), 8 x 32768 in e4m3 98 us (5.5 TB/s), 1 x 333
-// 8.6 us (the latency of one range and its join).
+// 48 ragged to 6000 69 us (5.7 TB/s), 8 x 32768 in e4m3 94 us (5.7 TB/s), 1 x 333
+// 8.1 us (the latency of one range and its join).
 #pragma once
 
 #include "fp8gq_device.cuh"

@@ -6,6 +6,10 @@
 // half and the 8 values they rotate with in the second half (two 16-byte
 // loads), so the rotation needs no exchange and the norm's sum of squares a
 // butterfly over D / 16 lanes.  fp32 throughout, one rounding at the store.
+//
+// Measured, 32 query and 8 kv heads of 128: 6001 tokens 32 us (151 MB, 4.7 TB/s),
+// 24 tokens into an e4m3 cache 2.6 us (the launch).  Four heads per group of lanes
+// took 39 us for the 6001.
 #pragma once
 
 #include "fp8gq_device.cuh"
