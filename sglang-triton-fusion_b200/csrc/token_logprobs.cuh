@@ -605,7 +605,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     if (lane == 0) s_regular = regular;
     if (regular) {
       const float l2s = log2f(sum.s);
-      auto logprob = [&](float x) { return kLn2 * (__fmaf_rn(x, kLog2e, -sum.m) - l2s); };
+      // x log2(e) of a value near the type's lowest (a mask) is past fp32 where x is
+      // not; next to such an x the roundings of r do not show
+      auto logprob = [&](float x) {
+        return x < kLpLowest ? x - kLn2 * (sum.m + l2s) : kLn2 * (__fmaf_rn(x, kLog2e, -sum.m) - l2s);
+      };
       if (lane == 0) {
         if (p.logprobs) p.logprobs[t] = token < 0 ? 0.0f : token >= p.V ? NAN : logprob(token_logit);
         if (p.entropy) p.entropy[t] = kLn2 * (l2s - sum.e / sum.s);
