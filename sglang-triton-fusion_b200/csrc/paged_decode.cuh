@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
   using Cfg = DecCfg<D, kFp8, kNT>;
   constexpr int kTok = Cfg::kTok, kTile = Cfg::kTile, kMT = D / 16, kKT = D / 16, kTT = kTok / 16;
   constexpr int kSlot = dec_slot_floats(D, kNT);
+  constexpr float kWeight = kFp8 ? 32768.0f : 1.0f;       // what a weight of 1 is as an operand
   constexpr int kRowK = Cfg::kRowK, kRowV = Cfg::kRowV;
   constexpr uint64_t kFull = kTok == 64 ? ~0ull : (1ull << (kTok & 63)) - 1;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -571,8 +572,10 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
             o[nt][i][3] *= a1;
           }
         }
-        // the weights meet v in v's 16-bit type (bf16; f16 for an e4m3 cache):
-        // each is off by half an ulp at most, their sum l is of the unrounded
+        // the weights meet v in 16 bits: bf16, each off by half an ulp at most; for
+        // an e4m3 cache f16 (v is exact in it), times 2^15, so that they are off by half
+        // an ulp down to 2^-29 of the maximum's and by 2^-40 of it below.  Their sum
+        // l is of the unrounded.
         const float b0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
 #pragma unroll
         for (int tt = 0; tt < kTT; ++tt) {
@@ -580,8 +583,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
           const float p2 = ex2(s[nt][tt][2] - b0), p3 = ex2(s[nt][tt][3] - b1);
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
-          pf[nt][tt][0] = movmatrix_t(pack2<kFp8>(p0, p1));
-          pf[nt][tt][1] = movmatrix_t(pack2<kFp8>(p2, p3));
+          pf[nt][tt][0] = movmatrix_t(pack2<kFp8>(p0 * kWeight, p1 * kWeight));
+          pf[nt][tt][1] = movmatrix_t(pack2<kFp8>(p2 * kWeight, p3 * kWeight));
         }
       }
       // ---- o^T += v^T p^T ----
@@ -655,8 +658,9 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
         for (int i = 0; i < kMT; ++i) {
           if constexpr (kFp8) {
             const int d = g * (D / 8) + 2 * i;
-            *reinterpret_cast<float2*>(so + d) = make_float2(o[nt][i][0], o[nt][i][2]);
-            *reinterpret_cast<float2*>(so + Cfg::kPad + d) = make_float2(o[nt][i][1], o[nt][i][3]);
+            constexpr float kBack = 1.0f / kWeight;
+            *reinterpret_cast<float2*>(so + d) = make_float2(o[nt][i][0] * kBack, o[nt][i][2] * kBack);
+            *reinterpret_cast<float2*>(so + Cfg::kPad + d) = make_float2(o[nt][i][1] * kBack, o[nt][i][3] * kBack);
           } else {
             const int d = 16 * i + g;
             so[d] = o[nt][i][0];

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from tests.test_serve_ops import check_logprobs, randn
+from tests.test_serve_ops import attend64, check_attention, check_logprobs, randn
 
 gpu = pytest.mark.gpu
 
@@ -41,3 +41,32 @@ def test_logprobs_lowest_values_beside_ordinary_ones(f, dtype, t, v):
         x[3, 11] = -math.inf
     r = check_logprobs(f, x, tokens, 20)
     assert r.logprobs.isfinite().all() and r.top_logprobs[0].isfinite().all()
+
+
+# ----------------------------------------------------------------- decode --
+def check_e4m3_decode(f, q, k, v, scale):
+    """q [1, Hq, D], k and v [N, Hkv, D] in pages of 16."""
+    n, hkv, d = k.shape
+    pages = (n + 15) // 16
+    cache = torch.zeros(2, pages * 16, hkv, d, device="cuda")
+    cache[0, :n], cache[1, :n] = k, v
+    kc, vc = (c.view(pages, 16, hkv, d).to(torch.float8_e4m3fn) for c in cache)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    out, lse = f.paged_decode_attention(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda"), scale=scale,
+                                        return_lse=True)
+    seen = torch.ones(1, n, dtype=torch.bool, device="cuda")
+    check_attention(out, lse, *attend64(q, kc.view(-1, hkv, d)[:n].double(), vc.view(-1, hkv, d)[:n].double(), scale, seen))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("drop", [5.0, 14.7, 20.3, 24.6, 26.0, 28.9])
+def test_decode_e4m3_faint_tokens_count(f, d, drop):
+    """One token in 16 has all the weight and v = 0, the others 2^-drop of it each
+    and v = 1: what they add is the output."""
+    n, hq, hkv = 1000, 8, 2
+    q = torch.zeros(1, hq, d, device="cuda", dtype=torch.bfloat16)
+    q[:, :, 0] = 1
+    k, v = torch.zeros(n, hkv, d, device="cuda"), torch.ones(n, hkv, d, device="cuda")
+    k[::16, :, 0], v[::16] = 8, 0
+    check_e4m3_decode(f, q, k, v, drop * math.log(2) / 8)
