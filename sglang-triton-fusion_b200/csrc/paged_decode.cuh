@@ -435,9 +435,9 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
     const int heads = min(8 * kNT, p.group - hb * 8 * kNT);
 
     // q as the B operand.  bf16: as it lies.  e4m3 cache: f16, scaled by a
-    // power of two so that a head's largest is in [1, 2) (exact; what falls
-    // below 2^-24 of it is lost), k steps in the order of the k rows' 16-byte
-    // chunks.
+    // power of two so that a head's largest is in [2^14, 2^15): exact down to
+    // 2^-28 of it, off by 2^-39 of it below.  k steps in the order of the k rows'
+    // 16-byte chunks.
     uint32_t qf[kNT][kKT][2];
     float sc[kNT][2];
 #pragma unroll
@@ -455,15 +455,16 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
         for (int k = 0; k < kRaw; ++k) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(raw[nt][k])), fabsf(bf16_hi(raw[nt][k]))));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // 2^e <= amax < 2^(e+1); e from the exponent field, kept where 2^-e is normal too
-        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        // 2^e <= amax < 2^(e+1); e from the exponent field, kept where 2^(14-e) and its
+        // inverse are normal (126 for amax >= 2^127: at most 65280 then, in f16's range)
+        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -112), 126);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
 #pragma unroll
         for (int k = 0; k < kKT; ++k) {
           qf[nt][k][0] = pack2<true>(bf16_lo(raw[nt][2 * k]) * down, bf16_hi(raw[nt][2 * k]) * down);
           qf[nt][k][1] = pack2<true>(bf16_lo(raw[nt][2 * k + 1]) * down, bf16_hi(raw[nt][2 * k + 1]) * down);
         }
-        const float up = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        const float up = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
         sc[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t4);
         sc[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
       }

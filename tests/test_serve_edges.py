@@ -70,3 +70,15 @@ def test_decode_e4m3_faint_tokens_count(f, d, drop):
     k, v = torch.zeros(n, hkv, d, device="cuda"), torch.ones(n, hkv, d, device="cuda")
     k[::16, :, 0], v[::16] = 8, 0
     check_e4m3_decode(f, q, k, v, drop * math.log(2) / 8)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("most", [2.0 ** 12, 2.0 ** 20, 2.0 ** 26])
+def test_decode_e4m3_one_large_query_value(f, d, most):
+    """A value of q that no key meets: the others give the scores, at full accuracy."""
+    n, hq, hkv = 700, 16, 2
+    q = randn(1, 1, hq, d).bfloat16()
+    k, v = randn(2, n, hkv, d, scale=2.0), randn(3, n, hkv, d)
+    q[:, :, 3], k[:, :, 3] = most, 0
+    check_e4m3_decode(f, q, k, v, d ** -0.5)
