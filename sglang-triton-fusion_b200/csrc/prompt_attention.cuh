@@ -640,9 +640,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
 #pragma unroll
           for (int y = 0; y < 8; ++y) mx8[y] = fmaxf(fmaxf(mx8[y], __uint_as_float(s[x + y])), __uint_as_float(s[x + 8 + y]));
         const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-        // O keeps its reference maximum until a row's grows by more than 2^60:
-        // fp32 and bf16 weights are as exact at any scale
-        const bool move = (mx - m) * c > 60.0f || (m == -INFINITY && mx > -INFINITY);
+        // O keeps its reference maximum until a row's weights would pass 2^8: they are
+        // as exact at any scale, but O has to stay in fp32's range with them
+        const bool move = (mx - m) * c > 8.0f || (m == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, move)) {
           const float mn = fmaxf(m, mx);
           if (j > 0) {

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from tests.test_serve_ops import attend64, check_attention, check_logprobs, randn
+from tests.test_serve_ops import attend64, check_attention, check_logprobs, check_prompt, prompt_case, randn
 
 gpu = pytest.mark.gpu
 
@@ -82,3 +82,18 @@ def test_decode_e4m3_one_large_query_value(f, d, most):
     k, v = randn(2, n, hkv, d, scale=2.0), randn(3, n, hkv, d)
     q[:, :, 3], k[:, :, 3] = most, 0
     check_e4m3_decode(f, q, k, v, d ** -0.5)
+
+
+# ----------------------------------------------------------------- prompt --
+@gpu
+@pytest.mark.parametrize("d, n", [(64, 300), (128, 300), (128, 4000)])
+def test_prompt_large_values_behind_a_growing_maximum(f, d, n):
+    """Scores that grow by 2^55 from one part of the keys to the next, and values of
+    1e25 or 1e30: the weighted sums stay in range as long as the values do."""
+    q = torch.zeros(40, 4, d, device="cuda")
+    q[:, :, 0] = 1
+    k, v = torch.zeros(n, 1, d, device="cuda"), randn(n, n, 1, d, scale=1e25)
+    k[n // 2:, :, 0] = 38.0
+    v[::7] *= 1e5
+    cu = lambda m: torch.tensor([0, m], dtype=torch.int32, device="cuda")  # noqa: E731
+    check_prompt(f, q.bfloat16(), k.bfloat16(), v.bfloat16(), cu(40), cu(n), scale=1.0)
