@@ -624,9 +624,18 @@ int fp8gq_paged_decode_attention(const void *q, int64_t q_token_stride, int64_t 
  * or NaN may reach the rows of its tile).  An offset out of range is cut to
  * [0, Tq] or [0, Tk] and recorded in the device error word.
  * workspace: fp8gq_prompt_workspace_bytes bytes (0 without a usable device), as
- * for fp8gq_paged_decode_attention.
+ * for fp8gq_paged_decode_attention.  A call with few items over long keys is
+ * split: it makes two launches, and the second reads what the first left in the
+ * workspace.  fp8gq_prompt_split_bytes says which calls are: it gives the bytes
+ * that such a call needs (not zero-filled), and 0 for one that makes one launch
+ * and needs FP8GQ_PROMPT_COUNTER_BYTES zero-filled ones.  From the start of a
+ * split call to its return nothing else may be launched on its workspace, so where
+ * several threads launch on one stream, or replay graphs there, it has a
+ * workspace of its own.
  * At most 128 query heads per kv head; scale is finite. */
+#define FP8GQ_PROMPT_COUNTER_BYTES 16384
 size_t fp8gq_prompt_workspace_bytes(void);
+size_t fp8gq_prompt_split_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int D, int causal);
 int fp8gq_prompt_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
                            const void *k, int64_t k_token_stride, int64_t k_head_stride,
                            const void *v, int64_t v_token_stride, int64_t v_head_stride,

@@ -33,7 +33,8 @@
 // list, go to the CTAs in equal ranges.  An item that lies in one range is
 // written as above; of one that lies in several, each CTA leaves its piece (O as
 // it is and the rows' m and l, fp32) in the workspace, and prompt_join_kernel
-// adds them in the order of the keys, rescaled to the largest m.
+// adds them in the order of the keys, rescaled to the largest m.  (Nothing else may
+// use that workspace between the two launches.)
 //
 // The two tiles' warps that share a scheduler take turns at the exponentials:
 // left alone they fall into step, both in the MUFU at half speed and then both
@@ -807,7 +808,12 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p) 
   grid_dependency_wait();
   const int c = blockIdx.x, d0 = 16 * blockIdx.y;
   const PrSplit e = p.splits[c];
-  if (e.last > c) {
+  // (records that something else has written to the workspace between the two
+  // launches, against the rule, do not become addresses)
+  const bool good = e.last < static_cast<int>(gridDim.x) && e.q0 >= 0 && e.lq >= 0 && e.lq <= p.Tq - e.q0 && e.r0 >= 0 &&
+                    e.r0 <= e.lq && e.hk >= 0 && e.hk < p.Hkv;
+  if (e.last > c && !good) record_error(kSiteBadIndex);
+  if (e.last > c && good) {
     const int i = threadIdx.x >> 7, row = threadIdx.x & 127;
     const int row_tok = (row * p.group_inv) >> 16, row_head = row - row_tok * p.group;
     const int tok = e.r0 + i * p.rows + row_tok;

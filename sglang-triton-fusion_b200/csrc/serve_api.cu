@@ -108,10 +108,12 @@ bool prompt_split(int B, int Tq, int Tk, int Hkv, int span, int keys, bool causa
   return (busiest - mean) * keys >= kPromptSplitGain;
 }
 
-size_t prompt_workspace_bytes(int sm_count) {
-  return kDecCounterBytes + sm_count * (sizeof(PrSplit) + 2 * sizeof(float) * PrCfg<128>::kPart);
+// Counters, and where a split call leaves its pieces.
+static_assert(FP8GQ_PROMPT_COUNTER_BYTES == kDecCounterBytes, "");
+size_t prompt_split_bytes(int D, int sm_count) {
+  return kDecCounterBytes + sm_count * (sizeof(PrSplit) + 2 * sizeof(float) * (D == 128 ? PrCfg<128>::kPart : PrCfg<64>::kPart));
 }
-
+int prompt_keys(int D) { return D == 128 ? PrCfg<128>::kKeys : PrCfg<64>::kKeys; }
 
 // [tokens, heads, D] bf16 as boxes of 64 values x `box_heads` heads x
 // `box_tokens` tokens, 128-byte swizzle.  A stride that no coordinate above 0
@@ -292,7 +294,16 @@ int fp8gq_paged_decode_attention(const void* q, int64_t q_token_stride, int64_t 
 size_t fp8gq_prompt_workspace_bytes(void) {
   DeviceInfo di;
   if (device_info(&di, nullptr) != FP8GQ_OK) return 0;
-  return prompt_workspace_bytes(di.sm_count);
+  return prompt_split_bytes(128, di.sm_count);
+}
+
+size_t fp8gq_prompt_split_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int D, int causal) {
+  DeviceInfo di;
+  if (B < 1 || Tq < 1 || Tk < 0 || check_heads(Hq, Hkv, D) != FP8GQ_OK || Hq / Hkv > 128 ||
+      device_info(&di, nullptr) != FP8GQ_OK ||
+      !prompt_split(B, Tq, Tk, Hkv, 2 * (128 / (Hq / Hkv)), prompt_keys(D), causal != 0, di.sm_count))
+    return 0;
+  return prompt_split_bytes(D, di.sm_count);
 }
 
 int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -335,7 +346,7 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
   p.scale_log2 = scale == 0.0f ? 1e-30f : std::fabs(scale) * 1.4426950408889634f;
   p.negate = scale < 0.0f;
   p.causal = causal ? 1 : 0;
-  const int keys = D == 128 ? PrCfg<128>::kKeys : PrCfg<64>::kKeys;
+  const int keys = prompt_keys(D);
   CUtensorMap tq, tk, tv;
   if (!make_heads_tmap(&tq, q, Tq, Hq, D, q_token_stride, q_head_stride, group, p.rows) ||
       !make_heads_tmap(&tk, Tk ? k : q, Tk ? Tk : 1, Hkv, D, Tk ? k_token_stride : 0, Tk ? k_head_stride : D, 1, keys) ||
@@ -344,12 +355,13 @@ int fp8gq_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head
   // a row block more than the tokens fill for each sequence's odd end
   const int64_t items = (static_cast<int64_t>(Tq) / (2 * p.rows) + B) * Hkv;
   if (items > INT32_MAX / 2) return FP8GQ_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < prompt_workspace_bytes(di.sm_count)) return FP8GQ_ERR_WORKSPACE;
+  p.split = prompt_split(B, Tq, Tk, Hkv, 2 * p.rows, keys, causal != 0, di.sm_count);
+  const size_t need = p.split ? prompt_split_bytes(D, di.sm_count) : FP8GQ_PROMPT_COUNTER_BYTES;
+  if (!workspace || workspace_bytes < need) return FP8GQ_ERR_WORKSPACE;
   if (!aligned16(workspace)) return FP8GQ_ERR_ALIGNMENT;
   p.counters = static_cast<int*>(workspace);
   p.splits = reinterpret_cast<PrSplit*>(static_cast<char*>(workspace) + kDecCounterBytes);
   p.parts = reinterpret_cast<float*>(p.splits + di.sm_count);
-  p.split = prompt_split(B, Tq, Tk, Hkv, 2 * p.rows, keys, causal != 0, di.sm_count);
   const unsigned blocks = static_cast<unsigned>(p.split || items > di.sm_count ? di.sm_count : items);
   auto fn = D == 128 ? prompt_attention_kernel<128> : prompt_attention_kernel<64>;
   const size_t smem = D == 128 ? PrCfg<128>::kSmem : PrCfg<64>::kSmem;

@@ -195,7 +195,17 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     cudaStream_t stream;
     void* ws;
     size_t ws_n;
-    if (!stream_of(dev, &stream) || !workspace(dev, stream, fp8gq_prompt_workspace_bytes(), &ws, &ws_n)) return not_here();
+    if (!stream_of(dev, &stream)) return not_here();
+    // a split call's scratch is its own: another thread's launch may come between its two
+    at::Tensor own;
+    ws_n = fp8gq_prompt_split_bytes(static_cast<int>(cq->size(0) - 1), static_cast<int>(tq), static_cast<int>(tk),
+                                    static_cast<int>(hq), static_cast<int>(hkv), static_cast<int>(d), a[5] == Py_True);
+    if (ws_n) {
+      own = empty({static_cast<int64_t>(ws_n)}, at::kByte, dev);
+      ws = own.data_ptr();
+    } else if (!workspace(dev, stream, FP8GQ_PROMPT_COUNTER_BYTES, &ws, &ws_n)) {
+      return not_here();
+    }
     const bool want_lse = a[7] == Py_True;
     const at::Tensor out = empty({tq, hq, d}, at::kBFloat16, dev);
     const at::Tensor lse = want_lse ? empty({tq, hq}, at::kFloat, dev) : at::Tensor();

@@ -149,6 +149,7 @@ SIGNATURES = {
     "fp8gq_prompt_attention": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P,
                                     _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P]),
     "fp8gq_prompt_workspace_bytes": (_SZ, []),
+    "fp8gq_prompt_split_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
     "fp8gq_token_logprobs": (_I, [_P, _I64, _I, _P, _I, _I, _P, _P, _P, _P, _I, _P]),
     "fp8gq_prepare_fused_gemv_quant": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _SZ,
                                             ctypes.POINTER(LaunchPlan)]),

@@ -26,9 +26,9 @@ from .ops import RMS_EPS, ShapeError, _check_cuda, _stream, _workspace_entry, _w
 
 HEAD_DIMS = (64, 128)
 MAX_TOP = 32
+PROMPT_COUNTER_BYTES = 16384   # FP8GQ_PROMPT_COUNTER_BYTES
 _BF16, _E4M3, _F32 = 0, 1, 2   # FP8GQ_DTYPE_*
 _byref = ctypes.byref
-_prompt_ws_bytes: dict = {}    # device -> fp8gq_prompt_workspace_bytes
 _decode_ws_bytes: dict = {}    # (device, Hq, Hkv, D) -> fp8gq_paged_decode_workspace_bytes
 
 
@@ -224,11 +224,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
             raise ShapeError(f"out must be {tuple(q.shape)}, got {tuple(shape)}")
     lse = torch.empty((tq, hq), dtype=torch.float32, device=dev) if return_lse else None
     stream = _stream(dev)
-    nbytes = _prompt_ws_bytes.get(dev.index)
-    if nbytes is None:
-        nbytes = _prompt_ws_bytes[dev.index] = _lib.load().fp8gq_prompt_workspace_bytes()
-    _, ws_ptr, ws_n = _workspace_entry(dev, nbytes, stream)
-    st = _lib.load().fp8gq_prompt_attention(
+    lib = _lib.load()
+    nbytes = lib.fp8gq_prompt_split_bytes(n - 1, tq, tk, hq, hkv, d, 1 if causal else 0)
+    if nbytes:      # two launches: scratch of this call's own, since another thread's launch may come between them
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws_ptr, ws_n = ws.data_ptr(), nbytes
+    else:
+        _, ws_ptr, ws_n = _workspace_entry(dev, PROMPT_COUNTER_BYTES, stream)
+    st = lib.fp8gq_prompt_attention(
         q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0],
         os[1], None if lse is None else lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), n - 1, tq, tk, hq, hkv, d,
         d ** -0.5 if scale is None else scale, 1 if causal else 0, ws_ptr, ws_n, stream)

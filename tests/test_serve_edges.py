@@ -97,3 +97,67 @@ def test_prompt_large_values_behind_a_growing_maximum(f, d, n):
     v[::7] *= 1e5
     cu = lambda m: torch.tensor([0, m], dtype=torch.int32, device="cuda")  # noqa: E731
     check_prompt(f, q.bfloat16(), k.bfloat16(), v.bfloat16(), cu(40), cu(n), scale=1.0)
+
+
+@gpu
+@pytest.mark.parametrize("with_out", [False, True])
+def test_prompt_split_call_has_scratch_of_its_own(f, with_out):
+    """A split call's two launches share nothing that another thread's launch between
+    them could use: the scratch of the stream is as it was."""
+    from fp8gq import ops
+    q, k, v, cu_q, cu_k = prompt_case(21, [64], [6000], 16, 1, 128)
+    dev, stream = torch.device("cuda", 0), torch.cuda.current_stream().cuda_stream
+    assert f._lib.load().fp8gq_prompt_split_bytes(1, q.shape[0], k.shape[0], 16, 1, 128, 1) > 0
+    scratch = ops.workspace(dev, 48 << 20, stream)
+    scratch[16384:] = 0x5a
+    out = torch.empty_like(q) if with_out else None
+    f.prompt_attention(q, k, v, cu_q, cu_k, out=out)
+    same = (scratch[16384:] == 0x5a).all() and (scratch[:16384] == 0).all()
+    scratch.zero_()
+    assert same
+
+
+@gpu
+def test_two_threads_on_one_stream(f):
+    """One thread's split prompts and another's decodes, linears and split prompts."""
+    import threading
+
+    from tests.test_serve_ops import decode_case
+    from tests.test_zz_no_alloc import _operands
+    q, k, v, cu_q, cu_k = prompt_case(22, [40, 3], [3100, 2500], 8, 2, 128)
+    q2, k2, v2, cu_q2, cu_k2 = prompt_case(23, [9], [4000], 4, 4, 64)
+    kc, vc, table, ln = decode_case(24, [3000, 50], 2, 128, 16, torch.bfloat16)
+    qd = randn(8, 2, 8, 128).bfloat16()
+    x, wq, ws = _operands(4, 4096, 6144, 1, "cuda")
+    calls = [lambda: f.prompt_attention(q, k, v, cu_q, cu_k), lambda: f.paged_decode_attention(qd, kc, vc, table, ln),
+             lambda: f.fused_gemv_quant(x, wq, ws), lambda: f.prompt_attention(q2, k2, v2, cu_q2, cu_k2)]
+    rows = [slice(0, 43), slice(None), slice(None), slice(0, 9)]
+    prev = f.set_tm_options(f.TM_WORKSPACE_SPLITK)
+    wrong, stream = [], torch.cuda.Stream()
+    try:
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            want = [c()[r].clone() for c, r in zip(calls, rows)]
+
+        def run(which, out):
+            with torch.cuda.stream(stream):
+                got = []
+                for _ in range(200):
+                    for i in which:
+                        if i == 0 and out:          # the path that lets go of the interpreter's lock
+                            o = torch.empty_like(q)
+                            f.prompt_attention(q, k, v, cu_q, cu_k, out=o)
+                        else:
+                            o = calls[i]()
+                        got.append((i, o))
+                wrong.extend(i for i, o in got if not torch.equal(o[rows[i]], want[i]))
+
+        threads = [threading.Thread(target=run, args=a) for a in (([0], True), ([1, 2, 3], False))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        f.set_tm_options(prev)
+    stream.synchronize()
+    assert not wrong
