@@ -2,8 +2,8 @@
 linears (norm + rotary + cache write, attention) and after the lm_head (log
 probabilities).  torch-tensor front end of libfp8gq, as ``ops``: dtypes,
 shapes and layouts are checked here, outputs come from torch's caching
-allocator, and the kernels run on torch's current stream.  There is no CPU
-path.
+allocator, and the kernels run on the tensors' device, on torch's current stream
+there.  There is no CPU path.
 
 A paged cache is two tensors ``k_cache`` and ``v_cache`` of shape [pages,
 page_size, kv heads, D], bf16 or float8_e4m3fn (a stored value then stands for
@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 
 from . import _build, _lib
-from .ops import RMS_EPS, ShapeError, _check_cuda, _stream, _workspace_entry, _workspaces
+from .ops import RMS_EPS, ShapeError, _stream, _workspace_entry, _workspaces
 
 HEAD_DIMS = (64, 128)
 MAX_TOP = 32
@@ -49,6 +49,21 @@ class _Binding:
 
 
 _native = _Binding()
+
+
+def _check_device(*ts):
+    """The one CUDA device that all of the tensors (None: not given) are on."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("fp8gq ops take CUDA tensors only (there is no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"all tensors must be on one device, got {dev} and {t.device}")
+    return dev
 
 
 def _check_cache(k, v, k_scale, v_scale):
@@ -110,7 +125,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch
                                         k_scale, v_scale, return_k)
         if r is not None:
             return r
-    _check_cuda(qkv, positions, slots, cos_sin, k_cache, v_cache, q_weight, k_weight, q_out, k_out)
+    dev = _check_device(qkv, positions, slots, cos_sin, k_cache, v_cache, q_weight, k_weight, q_out, k_out)
     cache, hkv, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise TypeError("qkv must be a 2-D bf16 tensor, contiguous along its last dimension")
@@ -125,17 +140,18 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None:
             _check_vector(w, name, d, torch.bfloat16)
-    q_out = _check_out(q_out, (t, hq, d), qkv.device)
+    q_out = _check_out(q_out, (t, hq, d), dev)
     if return_k or k_out is not None:
-        k_out = _check_out(k_out, (t, hkv, d), qkv.device)
+        k_out = _check_out(k_out, (t, hkv, d), dev)
     for o, name in ((q_out, "q_out"), (k_out, "k_out")):
         if o is not None and (o.stride(2) != 1 or (o.shape[1] > 1 and o.stride(1) != d)):
             raise ValueError(f"a token's heads must be contiguous in {name}")
-    st = _lib.load().fp8gq_qk_norm_rope_append(
-        qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
-        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
-        q_out.data_ptr(), q_out.stride(0), None if k_out is None else k_out.data_ptr(),
-        0 if k_out is None else k_out.stride(0), _byref(cache), t, hq, hkv, d, _stream(qkv.device))
+    with torch.cuda.device(dev):
+        st = _lib.load().fp8gq_qk_norm_rope_append(
+            qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+            q_out.data_ptr(), q_out.stride(0), None if k_out is None else k_out.data_ptr(),
+            0 if k_out is None else k_out.stride(0), _byref(cache), t, hq, hkv, d, _stream(dev))
     _lib.check(st, "fp8gq_qk_norm_rope_append")
     return (q_out, k_out) if return_k else q_out
 
@@ -153,7 +169,7 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         r = _native.paged_decode_attention(q, k_cache, v_cache, page_table, lens, scale, k_scale, v_scale, return_lse)
         if r is not None:
             return r
-    _check_cuda(q, k_cache, v_cache, page_table, lens, out)
+    dev = _check_device(q, k_cache, v_cache, page_table, lens, out)
     cache, hkv, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
     (b, hq, _), qs = _check_heads(q, "q", d)
     if hq % hkv:
@@ -162,7 +178,6 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b \
             or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ShapeError(f"page_table must be an int32 tensor [{b}, pages], contiguous along its last dimension")
-    dev = q.device
     if out is None:
         out = torch.empty((b, hq, d), dtype=torch.bfloat16, device=dev)
         os = (hq * d, d)
@@ -172,16 +187,17 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
             raise ShapeError(f"out must be {(b, hq, d)}, got {tuple(shape)}")
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     lib = _lib.load()
-    stream = _stream(dev)
-    key = (dev.index, hq, hkv, d)
-    nbytes = _decode_ws_bytes.get(key)
-    if nbytes is None:
-        nbytes = _decode_ws_bytes[key] = lib.fp8gq_paged_decode_workspace_bytes(hq, hkv, d)
-    _, ws_ptr, ws_n = _workspace_entry(dev, nbytes, stream)
-    st = lib.fp8gq_paged_decode_attention(
-        q.data_ptr(), qs[0], qs[1], _byref(cache), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-        lens.data_ptr(), out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(), b, hq, hkv, d,
-        d ** -0.5 if scale is None else scale, ws_ptr, ws_n, stream)
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        key = (dev.index, hq, hkv, d)
+        nbytes = _decode_ws_bytes.get(key)
+        if nbytes is None:
+            nbytes = _decode_ws_bytes[key] = lib.fp8gq_paged_decode_workspace_bytes(hq, hkv, d)
+        _, ws_ptr, ws_n = _workspace_entry(dev, nbytes, stream)
+        st = lib.fp8gq_paged_decode_attention(
+            q.data_ptr(), qs[0], qs[1], _byref(cache), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+            lens.data_ptr(), out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(), b, hq, hkv, d,
+            d ** -0.5 if scale is None else scale, ws_ptr, ws_n, stream)
     _lib.check(st, "fp8gq_paged_decode_attention")
     return (out, lse) if return_lse else out
 
@@ -199,7 +215,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         r = _native.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)
         if r is not None:
             return r
-    _check_cuda(q, k, v, cu_q, cu_k, out)
+    dev = _check_device(q, k, v, cu_q, cu_k, out)
     (tq, hq, d), qs = _check_heads(q, "q")
     (tk, hkv, _), ks = _check_heads(k, "k", d)
     vshape, vs = _check_heads(v, "v", d)
@@ -214,7 +230,6 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     n = cu_q.shape[0]
     _check_vector(cu_q, "cu_q", n, torch.int32)
     _check_vector(cu_k, "cu_k", n, torch.int32)
-    dev = q.device
     if out is None:
         out = torch.empty((tq, hq, d), dtype=torch.bfloat16, device=dev)
         os = (hq * d, d)
@@ -223,18 +238,19 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if shape != q.shape:
             raise ShapeError(f"out must be {tuple(q.shape)}, got {tuple(shape)}")
     lse = torch.empty((tq, hq), dtype=torch.float32, device=dev) if return_lse else None
-    stream = _stream(dev)
     lib = _lib.load()
-    nbytes = lib.fp8gq_prompt_split_bytes(n - 1, tq, tk, hq, hkv, d, 1 if causal else 0)
-    if nbytes:      # two launches: scratch of this call's own, since another thread's launch may come between them
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        ws_ptr, ws_n = ws.data_ptr(), nbytes
-    else:
-        _, ws_ptr, ws_n = _workspace_entry(dev, PROMPT_COUNTER_BYTES, stream)
-    st = lib.fp8gq_prompt_attention(
-        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0],
-        os[1], None if lse is None else lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), n - 1, tq, tk, hq, hkv, d,
-        d ** -0.5 if scale is None else scale, 1 if causal else 0, ws_ptr, ws_n, stream)
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        nbytes = lib.fp8gq_prompt_split_bytes(n - 1, tq, tk, hq, hkv, d, 1 if causal else 0)
+        if nbytes:      # two launches: scratch of this call's own, since another thread's launch may come between them
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws_ptr, ws_n = ws.data_ptr(), nbytes
+        else:
+            _, ws_ptr, ws_n = _workspace_entry(dev, PROMPT_COUNTER_BYTES, stream)
+        st = lib.fp8gq_prompt_attention(
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0],
+            os[1], None if lse is None else lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), n - 1, tq, tk, hq, hkv, d,
+            d ** -0.5 if scale is None else scale, 1 if causal else 0, ws_ptr, ws_n, stream)
     _lib.check(st, "fp8gq_prompt_attention")
     return (out, lse) if return_lse else out
 
@@ -255,7 +271,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     r = _native.token_logprobs(logits, tokens, top_k)
     if r is not None:
         return TokenLogprobs._make(r)
-    _check_cuda(logits, tokens)
+    dev = _check_device(logits, tokens)
     if logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2:
         raise TypeError("logits must be a 2-D bf16 or fp32 tensor")
     t, v = logits.shape
@@ -263,7 +279,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         raise ValueError("logits must be contiguous along the vocabulary")
     if not 0 <= top_k <= min(MAX_TOP, v):
         raise ShapeError(f"0 <= top_k <= {min(MAX_TOP, v)}, got {top_k}")
-    dev = logits.device
     lp = ids = tops = None
     if tokens is not None:
         _check_vector(tokens, "tokens", t, torch.int64)
@@ -271,9 +286,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     ent = torch.empty(t, dtype=torch.float32, device=dev)
     ids = torch.empty((t, top_k), dtype=torch.int64, device=dev)
     tops = torch.empty((t, top_k), dtype=torch.float32, device=dev)
-    st = _lib.load().fp8gq_token_logprobs(
-        logits.data_ptr(), logits.stride(0), _BF16 if logits.dtype == torch.bfloat16 else _F32,
-        None if tokens is None else tokens.data_ptr(), t, v, None if lp is None else lp.data_ptr(), ent.data_ptr(),
-        ids.data_ptr(), tops.data_ptr(), top_k, _stream(dev))
+    with torch.cuda.device(dev):
+        st = _lib.load().fp8gq_token_logprobs(
+            logits.data_ptr(), logits.stride(0), _BF16 if logits.dtype == torch.bfloat16 else _F32,
+            None if tokens is None else tokens.data_ptr(), t, v, None if lp is None else lp.data_ptr(), ent.data_ptr(),
+            ids.data_ptr(), tops.data_ptr(), top_k, _stream(dev))
     _lib.check(st, "fp8gq_token_logprobs")
     return TokenLogprobs(lp, ent, ids, tops)
