@@ -343,6 +343,11 @@ int fp8gq_device_error(uint32_t *code, int clear);
  * default in production.  FP8GQ_ERR_UNSUPPORTED for a limit out of range. */
 int fp8gq_set_wait_limit_ns(uint64_t limit_ns, uint64_t *previous);
 
+/* *id = a number of the graph capture that `stream` is in, the same throughout
+ * that capture, or 0 if it is in none.  A workspace zero-filled within a capture
+ * is zero-filled when that graph runs: it is of no use to another. */
+int fp8gq_capture_id(fp8gq_stream_t stream, uint64_t *id);
+
 /* Stack runner: a list of block-FP8 linears -- e.g. the qkv, o, gate_up and
  * down (SwiGLU) linears of every layer of a decode step -- run in list order
  * by ONE persistent, cooperative launch on all SMs.  Each linear is the tile

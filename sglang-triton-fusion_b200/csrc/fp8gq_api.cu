@@ -689,6 +689,19 @@ int fp8gq_set_wait_limit_ns(uint64_t limit_ns, uint64_t* previous) {
   return FP8GQ_OK;
 }
 
+int fp8gq_capture_id(fp8gq_stream_t stream, uint64_t* id) {
+  if (!id) return FP8GQ_ERR_NULL_POINTER;
+  *id = 0;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &n) != cudaSuccess) {
+    cudaGetLastError();      // (the legacy stream while another is captured: it is in none itself)
+    return FP8GQ_OK;
+  }
+  if (status == cudaStreamCaptureStatusActive) *id = n + 1;
+  return FP8GQ_OK;
+}
+
 int fp8gq_device_error(uint32_t* code, int clear) {
   if (!code) return FP8GQ_ERR_NULL_POINTER;
   unsigned int v = 0;

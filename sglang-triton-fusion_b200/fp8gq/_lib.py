@@ -111,6 +111,7 @@ SIGNATURES = {
     "fp8gq_fused_swiglu_q_gemm": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _SZ, _P]),
     "fp8gq_group_quant": (_I, [_P, _I64, _I, _I, _P, _P, _P]),
     "fp8gq_swiglu_group_quant": (_I, [_P, _I64, _I, _I, _P, _P, _P]),
+    "fp8gq_capture_id": (_I, [_P, ctypes.POINTER(ctypes.c_uint64)]),
     "fp8gq_device_error": (_I, [ctypes.POINTER(ctypes.c_uint32), _I]),
     "fp8gq_set_wait_limit_ns": (_I, [ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64)]),
     "fp8gq_add_rmsnorm": (_I, [_P, _I64, _P, _I64, _P, ctypes.c_float, _P, _I64, _P, _I64, _I, _I, _P]),

@@ -6,6 +6,8 @@ Every op runs the CUDA kernels; there is no CPU path.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -37,6 +39,7 @@ def _stream(device) -> int:
 
 _workspaces: dict = {}
 _outgrown: list = []    # scratch that a captured graph may still use
+_captured: dict = {}    # (device, stream) -> (capture, scratch that this capture made)
 _ws_bytes: dict = {}
 
 
@@ -52,8 +55,10 @@ def _workspace_bytes(lib, device, M, N, K, tile_only=False) -> int:
 
 def workspace(device: torch.device, nbytes: int, stream: int | None = None) -> torch.Tensor:
     """Zero-filled scratch kept per (device, stream).  The kernels leave it
-    zero-filled when they finish, so it is allocated and cleared once; grow it
-    (and warm every shape up) before capturing a CUDA graph."""
+    zero-filled when they finish, so it is allocated and cleared once.  A CUDA
+    graph captured on a stream without (enough) scratch gets its own, which the
+    graph clears each time that it runs: warm every shape up on the stream of the
+    capture to avoid that."""
     if stream is None:
         stream = _stream(device)
     return _workspace_entry(device, nbytes, stream)[0]
@@ -66,12 +71,34 @@ def _workspace_entry(device: torch.device, nbytes: int, stream: int):
     key = (device.index, stream)
     ent = _workspaces.get(key)
     if ent is None or ent[2] < nbytes:
-        if ent is not None:
-            _outgrown.append(ent[0])
-        buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        ent = (buf, buf.data_ptr(), buf.numel())
-        _workspaces[key] = ent
+        return _make_workspace(key, device, nbytes, stream)
     return ent
+
+
+def _make_workspace(key, device: torch.device, nbytes: int, stream: int):
+    def zeros():
+        buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        return buf, buf.data_ptr(), buf.numel()
+
+    capture = _capture_id(stream)
+    if capture:
+        # the zeros are only recorded: they are there for this graph, when it runs
+        held = _captured.get(key)
+        if held is None or held[0] != capture or held[1][2] < nbytes:
+            held = _captured[key] = (capture, zeros())
+        return held[1]
+    ent = _workspaces.get(key)
+    if ent is not None:
+        _outgrown.append(ent[0])
+    ent = _workspaces[key] = zeros()
+    return ent
+
+
+def _capture_id(stream: int) -> int:
+    """The graph capture that the stream is in, 0 if none."""
+    n = ctypes.c_uint64(0)
+    _lib.check(_lib.load().fp8gq_capture_id(stream, ctypes.byref(n)), "fp8gq_capture_id")
+    return n.value
 
 
 def _check_cuda(*ts):
