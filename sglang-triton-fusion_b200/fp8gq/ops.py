@@ -7,6 +7,7 @@ Every op runs the CUDA kernels; there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -39,6 +40,7 @@ def _stream(device) -> int:
 
 _workspaces: dict = {}
 _outgrown: list = []    # scratch that a captured graph may still use
+_workspace_lock = threading.Lock()
 _captured: dict = {}    # (device, stream) -> (capture, scratch that this capture made)
 _ws_bytes: dict = {}
 
@@ -87,11 +89,13 @@ def _make_workspace(key, device: torch.device, nbytes: int, stream: int):
         if held is None or held[0] != capture or held[1][2] < nbytes:
             held = _captured[key] = (capture, zeros())
         return held[1]
-    ent = _workspaces.get(key)
-    if ent is not None:
-        _outgrown.append(ent[0])
-    ent = _workspaces[key] = zeros()
-    return ent
+    with _workspace_lock:        # (threads that share a stream share its scratch)
+        ent = _workspaces.get(key)
+        if ent is None or ent[2] < nbytes:
+            if ent is not None:
+                _outgrown.append(ent[0])
+            ent = _workspaces[key] = zeros()
+        return ent
 
 
 def _capture_id(stream: int) -> int:

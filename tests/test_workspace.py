@@ -47,6 +47,28 @@ def test_scratch_of_a_capture_is_that_graphs_alone(fresh, monkeypatch):
     assert ops._workspace_entry(CPU, 100, 3) is c and ops._workspace_entry(CPU, 4 << 20, 3) is not d
 
 
+def test_threads_get_the_same_scratch(fresh, monkeypatch):
+    """Two threads' first calls on a stream: neither's scratch may be dropped while
+    its call is about to use it."""
+    import threading
+    zeros, inside = torch.zeros, threading.Barrier(2)
+
+    def slow(*a, **kw):
+        try:
+            inside.wait(0.5)             # both in here at once, if they can be
+        except threading.BrokenBarrierError:
+            pass
+        return zeros(*a, **kw)
+    monkeypatch.setattr(torch, "zeros", slow)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(ops._workspace_entry(CPU, 100, 3))) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got[0] is got[1] is ops._workspaces[(None, 3)]
+
+
 def test_no_capture_without_a_gpu():
     assert ops._capture_id(0) == 0
 
