@@ -78,6 +78,12 @@ bool workspace(int device, cudaStream_t stream, size_t bytes, void** p, size_t* 
   return !PyErr_Occurred() && *n >= bytes;
 }
 
+// A flag, True or False; anything else counts by its truth in serve.py.
+bool flag(PyObject* o, bool* v) {
+  *v = o == Py_True;
+  return PyBool_Check(o);
+}
+
 at::Tensor empty(c10::IntArrayRef sizes, at::ScalarType type, int device) {
   return at::empty(sizes, at::TensorOptions().dtype(type).device(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device))));
 }
@@ -127,9 +133,9 @@ PyObject* qk_norm_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[6] != Py_None && !(qw = vector(a[6], at::kBFloat16, d, &dev))) return not_here();
     if (a[7] != Py_None && !(kw = vector(a[7], at::kBFloat16, d, &dev))) return not_here();
     double eps;
+    bool want_k;
     cudaStream_t stream;
-    if (!number(a[8], &eps) || !stream_of(dev, &stream)) return not_here();
-    const bool want_k = a[11] == Py_True;
+    if (!number(a[8], &eps) || !flag(a[11], &want_k) || !stream_of(dev, &stream)) return not_here();
     const at::Tensor q = empty({t, hq, d}, at::kBFloat16, dev);
     const at::Tensor ko = want_k ? empty({t, hkv, d}, at::kBFloat16, dev) : at::Tensor();
     if (fp8gq_qk_norm_rope_append(qkv->data_ptr(), qkv->stride(0), pos->data_ptr<int64_t>(), slots->data_ptr<int64_t>(),
@@ -156,14 +162,14 @@ PyObject* paged_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *table = cuda_tensor(a[3], at::kInt, 2, &dev), *lens = vector(a[4], at::kInt, b, &dev);
     if (!table || !lens || table->size(0) != b || (table->size(1) > 1 && table->stride(1) != 1)) return not_here();
     double scale = 1.0 / std::sqrt(static_cast<double>(d));
-    if (a[5] != Py_None && !number(a[5], &scale)) return not_here();
+    bool want_lse;
+    if ((a[5] != Py_None && !number(a[5], &scale)) || !flag(a[8], &want_lse)) return not_here();
     cudaStream_t stream;
     void* ws;
     size_t ws_n;
     if (!stream_of(dev, &stream)) return not_here();
     const size_t need = fp8gq_paged_decode_workspace_bytes(static_cast<int>(hq), static_cast<int>(hkv), static_cast<int>(d));
     if (!workspace(dev, stream, need, &ws, &ws_n)) return not_here();
-    const bool want_lse = a[8] == Py_True;
     const at::Tensor out = empty({b, hq, d}, at::kBFloat16, dev);
     const at::Tensor lse = want_lse ? empty({b, hq}, at::kFloat, dev) : at::Tensor();
     if (fp8gq_paged_decode_attention(q->data_ptr(), q->stride(0), q->stride(1), &c, table->data_ptr<int32_t>(),
@@ -191,7 +197,8 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!cq || cq->size(0) < 1 || !cq->is_contiguous()) return not_here();
     const at::Tensor* ck = a[4] == Py_None ? cq : vector(a[4], at::kInt, cq->size(0), &dev);
     double scale = 1.0 / std::sqrt(static_cast<double>(d));
-    if (!ck || !PyBool_Check(a[5]) || (a[6] != Py_None && !number(a[6], &scale))) return not_here();
+    bool causal, want_lse;
+    if (!ck || !flag(a[5], &causal) || !flag(a[7], &want_lse) || (a[6] != Py_None && !number(a[6], &scale))) return not_here();
     cudaStream_t stream;
     void* ws;
     size_t ws_n;
@@ -199,14 +206,13 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     // a split call's scratch is its own: another thread's launch may come between its two
     at::Tensor own;
     ws_n = fp8gq_prompt_split_bytes(static_cast<int>(cq->size(0) - 1), static_cast<int>(tq), static_cast<int>(tk),
-                                    static_cast<int>(hq), static_cast<int>(hkv), static_cast<int>(d), a[5] == Py_True);
+                                    static_cast<int>(hq), static_cast<int>(hkv), static_cast<int>(d), causal);
     if (ws_n) {
       own = empty({static_cast<int64_t>(ws_n)}, at::kByte, dev);
       ws = own.data_ptr();
     } else if (!workspace(dev, stream, FP8GQ_PROMPT_COUNTER_BYTES, &ws, &ws_n)) {
       return not_here();
     }
-    const bool want_lse = a[7] == Py_True;
     const at::Tensor out = empty({tq, hq, d}, at::kBFloat16, dev);
     const at::Tensor lse = want_lse ? empty({tq, hq}, at::kFloat, dev) : at::Tensor();
     if (fp8gq_prompt_attention(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1),
@@ -214,7 +220,7 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                want_lse ? lse.data_ptr<float>() : nullptr, cq->data_ptr<int32_t>(), ck->data_ptr<int32_t>(),
                                static_cast<int>(cq->size(0) - 1), static_cast<int>(tq), static_cast<int>(tk),
                                static_cast<int>(hq), static_cast<int>(hkv), static_cast<int>(d), static_cast<float>(scale),
-                               a[5] == Py_True, ws, ws_n, stream) != FP8GQ_OK)
+                               causal, ws, ws_n, stream) != FP8GQ_OK)
       return not_here();
     return want_lse ? pair(out, lse) : wrap(out);
   });

@@ -4,6 +4,7 @@ Bounds are those of test_serve_ops.py, derived there from the kernels' roundings
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -161,3 +162,27 @@ def test_two_threads_on_one_stream(f):
         f.set_tm_options(prev)
     stream.synchronize()
     assert not wrong
+
+
+# ------------------------------------------------------------------ flags --
+@gpu
+@pytest.mark.parametrize("yes", [1, np.bool_(True), "yes"])
+@pytest.mark.parametrize("no", [0, np.bool_(False), None])
+def test_flags_by_truth(f, yes, no):
+    """return_lse, return_k and causal count by their truth, as everywhere in Python."""
+    q, k, v, cu, _ = prompt_case(3, [5, 4], [5, 4], 4, 2, 64, spare=0)
+    out, lse = f.prompt_attention(q, k, v, cu, return_lse=yes)
+    assert out.shape == (9, 4, 64) and lse.shape == (9, 4)
+    assert torch.equal(f.prompt_attention(q, k, v, cu, return_lse=no), out)
+    assert torch.equal(f.prompt_attention(q, k, v, cu, causal=yes), out)
+    assert torch.equal(f.prompt_attention(q, k, v, cu, causal=no), f.prompt_attention(q, k, v, cu, causal=False))
+    kc = randn(4, 3, 4, 2, 64).bfloat16()
+    table, lens = torch.tensor([[0, 1], [2, 1]], dtype=torch.int32, device="cuda"), torch.tensor([5, 8], dtype=torch.int32, device="cuda")
+    o, s = f.paged_decode_attention(q[:2], kc, kc, table, lens, return_lse=yes)
+    assert o.shape == (2, 4, 64) and s.shape == (2, 4)
+    assert torch.equal(f.paged_decode_attention(q[:2], kc, kc, table, lens, return_lse=no), o)
+    qkv, at = randn(5, 2, 8 * 64).bfloat16(), torch.arange(2, device="cuda")
+    cs = torch.ones(4, 64, device="cuda")
+    a, b = f.qk_norm_rope_append(qkv, at, at, cs, kc, kc.clone(), return_k=yes)
+    assert a.shape == (2, 4, 64) and b.shape == (2, 2, 64)
+    assert torch.equal(f.qk_norm_rope_append(qkv, at, at, cs, kc, kc.clone(), return_k=no), a)
