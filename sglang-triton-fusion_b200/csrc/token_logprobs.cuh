@@ -428,8 +428,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     bulk_g2s(ring + stage * kLpStepBytes, vec + v_lo + i * kStep, 16 * n, &s_full[stage], policy);
   };
   bool ok = true;
+  int sent = 0;                                  // thread 0: steps on their way or there
   if (tid == 0)
-    for (int i = 0; i < min(kLpStages, its); ++i) copy(i, i);
+    for (; sent < min(kLpStages, its); ++sent) copy(sent, sent);
   // the given token's logit, fetched meanwhile
   int64_t token = -1;
   float token_logit = 0.0f;
@@ -442,14 +443,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   uint32_t phase = 0;
   for (int i = 0; i < its; ++i) {
     LpChunk<T> now;
-    ok = mbar_wait_warp(&s_full[stage], phase, kSiteScore, lane) && ok;
-    now.load(smem_u32(ring) + stage * kLpStepBytes, warp * 32 * kLpUnroll + lane, ok ? v_hi - v_lo - i * kStep : 0);
+    ok = mbar_wait_warp(&s_full[stage], phase, kSiteScore, lane);
+    if (!ok) break;
+    now.load(smem_u32(ring) + stage * kLpStepBytes, warp * 32 * kLpUnroll + lane, v_hi - v_lo - i * kStep);
     __syncwarp();
     if (lane == 0) mbar_arrive(&s_free[stage]);
-    // the stage of the step before, which every warp has read by now or soon
-    if (tid == 0 && i > 0 && i - 1 + kLpStages < its) {
+    // the stage of the step before, which every warp has read by now or soon (unless
+    // one gave up: then nothing more is sent)
+    if (tid == 0 && i > 0 && sent == i - 1 + kLpStages && sent < its) {
       const int before_stage = stage == 0 ? kLpStages - 1 : stage - 1;
-      if (mbar_wait(&s_free[before_stage], stage == 0 ? phase ^ 1 : phase, kSiteScore)) copy(i - 1 + kLpStages, before_stage);
+      if (mbar_wait(&s_free[before_stage], stage == 0 ? phase ^ 1 : phase, kSiteScore)) copy(sent++, before_stage);
     }
     if (++stage == kLpStages) {
       stage = 0;
@@ -480,10 +483,19 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   sum.s = s2.x + s2.y;
   sum.e = e2.x + e2.y;
 
+  // where a wait gave up, the copies sent land before the ring takes the candidates
+  // or goes to another CTA, and the row is done again as an irregular one
+  const bool gave_up = __syncthreads_or(!ok) != 0;           // (the ring has been read)
+  if (gave_up) {
+    if (tid == 0)
+      for (int i = max(sent - kLpStages, 0); i < sent; ++i) mbar_wait(&s_full[i % kLpStages], (i / kLpStages) & 1, kSiteScore);
+    sum.s = NAN;
+    __syncthreads();
+  }
+
   // the candidates
   float low = -INFINITY;
-  if (K > 0) {
-    __syncthreads();                             // the ring has been read
+  if (K > 0 && !gave_up) {
     low = just_below(float_order(lp_kth(most, K, found.max, warp, lane)));
     // the columns to read again, listed (in any order)
     unsigned is[kLpParts];

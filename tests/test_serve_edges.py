@@ -186,3 +186,29 @@ def test_flags_by_truth(f, yes, no):
     a, b = f.qk_norm_rope_append(qkv, at, at, cs, kc, kc.clone(), return_k=yes)
     assert a.shape == (2, 4, 64) and b.shape == (2, 2, 64)
     assert torch.equal(f.qk_norm_rope_append(qkv, at, at, cs, kc, kc.clone(), return_k=no), a)
+
+
+# ----------------------------------------------------------- bounded waits --
+@pytest.fixture
+def shortest_limit(f):
+    """Every bounded wait at its shortest limit (2 ms inside a kernel)."""
+    torch.cuda.synchronize()
+    prev = f.set_wait_limit_ns(1_000_000)
+    yield
+    torch.cuda.synchronize()
+    f.set_wait_limit_ns(prev)
+    f.device_error(clear=True)
+
+
+@gpu
+@pytest.mark.parametrize("t, v, k", [(1, 151936, 32), (37, 151936, 20), (700, 50257, 0), (1500, 4099, 3)])
+def test_logprobs_under_the_shortest_limit(f, shortest_limit, t, v, k):
+    """No ordinary wait comes near the limit, so none is given up, whatever the
+    number of steps; the same row twice gives the same bits."""
+    x = randn(t, t, v, scale=3.0)
+    tokens = torch.arange(t, device="cuda") % v
+    r = f.token_logprobs(x, tokens, top_k=k)
+    torch.cuda.synchronize()
+    assert f.device_error() == 0
+    check_logprobs(f, x[:40], tokens[:40], k)
+    assert all(torch.equal(a, b) for a, b in zip(r, f.token_logprobs(x, tokens, top_k=k)))
