@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
   __shared__ uint64_t b_full[kSlots], b_free[kSlots];
   __shared__ uint64_t b_s[2], b_r[2], b_p[2], b_o[2];        // scores ready, read; weights ready; O updated
   __shared__ uint64_t b_out[2];                              // O read
-  __shared__ uint64_t b_end[2];                              // after a wait gave up: the products issued are done
+  __shared__ uint64_t b_end[2];                              // at the end: the products issued are done
   __shared__ uint64_t b_turn[2][4];                          // tile i's warp may have the MUFU
   __shared__ uint32_t s_tmem;
   __shared__ PrWork s_work[kPrItems];
@@ -466,6 +466,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
       // ---- TMA ----
       int x0 = 0, items = 0, tails = 0;             // k and v tiles, items and tails so far
       int q_sent = 0, sent = 0;                     // q, k and v tiles on their way or there
+      bool tail_sent = false;                       // the last of them is a v tile whose copy b_tail counts
       while (next_item()) {
         const int n = max(w.n[0], w.n[1]);
         const bool partial = n * kKeys > w.lk;      // the last tile reaches past the sequence
@@ -485,8 +486,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             if (x >= kSlots) ok = pr_wait_warp(&b_free[slot], (x / kSlots - 1) & 1);
             if (!ok) break;
             ++sent;
+            tail_sent = partial && i == 2 * n - 1;
             if (pr_elect()) {
-              uint64_t* bar = partial && i == 2 * n - 1 ? &b_tail : &b_full[slot];
+              uint64_t* bar = tail_sent ? &b_tail : &b_full[slot];
               mbar_arrive_expect_tx(bar, kTile);
               for (int h = 0; h < Cfg::kHalves; ++h)
                 tma_load_3d(ring + slot * kTile + h * Cfg::kHalf, (i & 1) ? &tv : &tk, 64 * h, w.hk, w.k0 + (i >> 1) * kKeys, bar);
@@ -506,6 +508,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&b_full[slot]);
+            tail_sent = false;
             ++tails;
           }
           x0 += 2 * n;
@@ -515,11 +518,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         if (lane == 0) mbar_arrive(&b_want);
         leave_item();
       }
-      // the copies that no one has waited for have landed before the CTA ends
-      // (only after a wait gave up: otherwise every tile has been used)
-      if (!ok && lane == 0) {
+      // every copy has landed before the CTA ends, whichever role gave a wait up
+      // (where none did, every tile is used and this waits for nothing else)
+      if (lane == 0) {
         if (q_sent) pr_wait(&b_q, (q_sent - 1) & 1);
-        for (int x = max(sent - kSlots, 0); x < sent; ++x) pr_wait(&b_full[x % kSlots], (x / kSlots) & 1);
+        for (int x = max(sent - kSlots, 0); x < sent; ++x) {
+          if (tail_sent && x == sent - 1) pr_wait(&b_tail, tails & 1);
+          else pr_wait(&b_full[x % kSlots], (x / kSlots) & 1);
+        }
       }
     } else {
       // ---- MMA of tile i: the warp waits together, one lane issues ----
@@ -585,11 +591,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
         if (mine > 0) ++outs;
         leave_item();
       }
-      if (!ok) {                                           // what has been issued completes
-        if (pr_elect()) mma_commit(&b_end[i]);
-        __syncwarp();
-        pr_wait_warp(&b_end[i], 0);
-      }
+      // what has been issued completes before the CTA ends, whichever role gave up
+      if (pr_elect()) mma_commit(&b_end[i]);
+      __syncwarp();
+      pr_wait_warp(&b_end[i], 0);
     }
   } else {
     // ---- softmax and output: one thread per row ----
@@ -789,6 +794,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
             l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m * c) + log2f(l)) * 0.6931471805599453f;
       leave_item();
     }
+    tmem_wait_st();                                        // (stores of a step that was given up)
     tc_fence_before();
   }
   __syncthreads();

@@ -212,3 +212,32 @@ def test_logprobs_under_the_shortest_limit(f, shortest_limit, t, v, k):
     assert f.device_error() == 0
     check_logprobs(f, x[:40], tokens[:40], k)
     assert all(torch.equal(a, b) for a, b in zip(r, f.token_logprobs(x, tokens, top_k=k)))
+
+
+@gpu
+@pytest.mark.parametrize("d, keys", [(128, 400_000), (64, 700_000)])
+@pytest.mark.parametrize("rounds", [1, 2])
+def test_prompt_items_longer_than_the_limit(f, shortest_limit, d, keys, rounds):
+    """Whole items that take longer than the limit (some 6 ms against 2): the wait for the next
+    item is given up and reported, the call ends, and the next one is right."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert sms % 4 == 0
+    n = rounds * sms // 4 * 256                            # an item for each SM and round
+    q = randn(1, n, 4, d).bfloat16()
+    k, v = randn(2, keys, 4, d).bfloat16(), randn(3, keys, 4, d).bfloat16()
+    cu = lambda m: torch.tensor([0, m], dtype=torch.int32, device="cuda")  # noqa: E731
+    cu_q, cu_k = cu(n), cu(keys)
+    assert f._lib.load().fp8gq_prompt_split_bytes(1, n, keys, 4, 4, d, 0) == 0
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    out = f.prompt_attention(q, k, v, cu_q, cu_k, causal=False)
+    end.record()
+    end.synchronize()
+    assert f.device_error(clear=True) == 0x80000000 | 11
+    assert start.elapsed_time(end) < 100
+    # the items that were begun are whole: the last rows of the sequence are the first
+    check_attention(out[-40:, 1:2], None, *attend64(q[-40:, 1:2], k[:, 1:2], v[:, 1:2], d ** -0.5,
+                                                    torch.ones(40, keys, dtype=torch.bool, device="cuda")))
+    a, b, c, cu_a, _ = prompt_case(5, [900, 77, 2000], [900, 77, 2000], 8, 2, d)
+    check_prompt(f, a, b, c, cu_a, None)
+    assert f.device_error() == 0
