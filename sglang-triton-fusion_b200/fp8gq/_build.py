@@ -1,6 +1,8 @@
 """Build libfp8gq.so (the C ABI in include/fp8gq.h) in-tree with nvcc for
-sm_100a, and the serving operators' Python binding next to it with g++.  Run ``python -m fp8gq._build`` (with ``sglang-triton-fusion_b200``
-on sys.path) or call :func:`build`."""
+sm_100a, and the serving operators' Python binding next to it with g++.  Run
+``python -m fp8gq._build`` (with ``sglang-triton-fusion_b200`` on sys.path) or
+call :func:`build`.  The library depends on no torch; the binding is of one torch
+and Python version, which its name tells, and the operators run without it."""
 from __future__ import annotations
 
 import os
@@ -20,7 +22,6 @@ HEADERS = {"fp8gq_api.cu": ["fp8gq_device.cuh", "host_common.h", "tensor_core.cu
                             "paged_decode.cuh", "prompt_attention.cuh", "token_logprobs.cuh"]}
 OBJ_DIR = PKG_DIR / "build"
 NATIVE_SOURCE = "serve_python.cpp"               # the serving operators' Python binding
-NATIVE_PATH = PKG_DIR / "_serve_native.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -48,12 +49,22 @@ def _newer_than(target: Path, files) -> bool:
     return all(f.stat().st_mtime <= t for f in files)
 
 
-def _native_inputs():
-    return [SRC_DIR / NATIVE_SOURCE, REPO_DIR / "include" / "fp8gq.h"]
+def native_path() -> Path:
+    """The binding for this torch and Python."""
+    import torch
+    return PKG_DIR / f"_serve_native-torch{torch.__version__}-py{sys.version_info[0]}.{sys.version_info[1]}.so"
+
+
+def library_up_to_date() -> bool:
+    return _newer_than(LIB_PATH, [f for s in SOURCES for f in _inputs(s)])
+
+
+def native_up_to_date() -> bool:
+    return _newer_than(native_path(), [SRC_DIR / NATIVE_SOURCE, REPO_DIR / "include" / "fp8gq.h"])
 
 
 def up_to_date() -> bool:
-    return _newer_than(LIB_PATH, [f for s in SOURCES for f in _inputs(s)]) and _newer_than(NATIVE_PATH, _native_inputs())
+    return library_up_to_date() and native_up_to_date()
 
 
 def _native_command(target: str):
@@ -73,9 +84,28 @@ def _native_command(target: str):
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
+    """Compile libfp8gq.so and the binding, whatever is not already current."""
+    build_library(force, verbose, extra_flags)
+    build_native(force)
+    return LIB_PATH
+
+
+def build_native(force: bool = False) -> Path:
+    """Compile the binding next to this file unless it is already current."""
+    path = native_path()
+    if force or not native_up_to_date():
+        tmp = f"{path}.{os.getpid()}.tmp"
+        res = subprocess.run(_native_command(tmp), capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        os.replace(tmp, path)
+    return path
+
+
+def build_library(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
     """Compile libfp8gq.so next to this file unless it is already current: one
     object per translation unit, in parallel, those that are current reused."""
-    if not force and up_to_date():
+    if not force and library_up_to_date():
         return LIB_PATH
     OBJ_DIR.mkdir(exist_ok=True)
     jobs = []
@@ -100,11 +130,6 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     os.replace(str(LIB_PATH) + ".tmp", LIB_PATH)
-    if force or not _newer_than(NATIVE_PATH, _native_inputs()):
-        res = subprocess.run(_native_command(str(NATIVE_PATH) + ".tmp"), capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError(f"g++ failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-        os.replace(str(NATIVE_PATH) + ".tmp", NATIVE_PATH)
     return LIB_PATH
 
 

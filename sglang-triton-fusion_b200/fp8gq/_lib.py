@@ -189,9 +189,9 @@ def load(build_if_missing: bool = True):
         if _lib is not None:
             return _lib
         path = _build.LIB_PATH
-        if build_if_missing and not _build.up_to_date():
+        if build_if_missing and not _build.library_up_to_date():
             try:
-                _build.build()
+                _build.build_library()
             except RuntimeError:
                 if not path.exists():
                     raise

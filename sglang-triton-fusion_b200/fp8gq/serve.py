@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -35,17 +36,31 @@ _decode_ws_bytes: dict = {}    # (device, Hq, Hkv, D) -> fp8gq_paged_decode_work
 class _Binding:
     """The C++ binding (csrc/serve_python.cpp), loaded at the first call.  Its
     functions return None for anything but the plain form of the arguments; the
-    checks below then raise, or complete the call."""
+    checks below then raise, or complete the call.  Where it can be neither loaded
+    nor built, they complete every call."""
 
     def __getattr__(self, name):
         _lib.load()
-        loader = importlib.machinery.ExtensionFileLoader("_serve_native", str(_build.NATIVE_PATH))
-        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_serve_native", loader))
-        loader.exec_module(mod)
-        mod.set_workspaces(_workspaces)
+        try:
+            loader = importlib.machinery.ExtensionFileLoader("_serve_native", str(_build.build_native()))
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_serve_native", loader))
+            loader.exec_module(mod)
+            mod.set_workspaces(_workspaces)
+        except (ImportError, OSError, RuntimeError) as e:
+            warnings.warn("fp8gq: the serving operators run without their C++ binding, 10 us more a call: "
+                          f"{str(e).strip()}", RuntimeWarning)
+            mod = _NoBinding()
         global _native
         _native = mod
         return getattr(mod, name)
+
+
+class _NoBinding:
+    @staticmethod
+    def _step_aside(*args):
+        return None
+
+    qk_norm_rope_append = paged_decode_attention = prompt_attention = token_logprobs = _step_aside
 
 
 _native = _Binding()
