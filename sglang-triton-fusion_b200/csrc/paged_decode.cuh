@@ -172,6 +172,10 @@ __device__ __forceinline__ int dec_len(const DecodeParams& p, int b, bool record
   return n;
 }
 
+// Tiles of a sequence of len > 0 tokens (any: no sum here passes 2^31 - 1).
+template <int kTile>
+__device__ __forceinline__ int dec_tiles(int len) { return (len - 1) / kTile + 1; }
+
 // N values of head h's output from their sum v and the weights' sum l (relative
 // to the maximum m); l = 0 where no token counted.
 template <int N>
@@ -223,7 +227,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
   int64_t mine = 0;
   for (int b = b_lo; b < b_hi; ++b) {
     const int len = dec_len(p, b, blockIdx.x == 0);
-    if (len > 0) mine += (len + kTile - 1) / kTile + kDecItemCost;
+    if (len > 0) mine += dec_tiles<kTile>(len) + kDecItemCost;
   }
   mine *= items;
   int64_t incl = mine;
@@ -269,7 +273,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
   auto owner = [&](int64_t t) { return static_cast<int>(quotient((t + 1) * ctas - 1, total)); };
 
   auto enter = [&](DecWalk& w) {              // w.b, w.sub and w.start are set
-    w.n = (w.len + kTile - 1) / kTile;
+    w.n = dec_tiles<kTile>(w.len);
     const int64_t first = w.start + kDecItemCost;
     w.j = t0 > first ? static_cast<int>(t0 - first) : 0;
     w.j_end = t1 - first < w.n ? static_cast<int>(t1 - first) : w.n;
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
     int b = lo * share, per = 0;
     for (;; ++b) {
       cur.len = dec_len(p, b, false);
-      per = cur.len > 0 ? (cur.len + kTile - 1) / kTile + kDecItemCost : 0;
+      per = cur.len > 0 ? dec_tiles<kTile>(cur.len) + kDecItemCost : 0;
       const int64_t here = static_cast<int64_t>(per) * items;
       if (t0 < at + here) break;
       at += here;
@@ -327,13 +331,14 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
     id_left = 0;
     if (pre.done) return;
     id_head = pre.sub / p.blocks;
-    const int base = pre.j * kTile + warp * kTok;
-    id_left = pre.len - base;
+    // (past the last token of a sequence of nearly 2^31 the first wraps, unused)
+    const unsigned base = static_cast<unsigned>(pre.j) * kTile + warp * kTok;
+    id_left = pre.len - pre.j * kTile - warp * kTok;
 #pragma unroll
     for (int i = 0; i < kIds; ++i) {
       const int r = lane + 32 * i;
       if (r < kTok && r < id_left) {
-        const int tok = base + r;
+        const int tok = static_cast<int>(base + r);
         const int c = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.cache.page_size;
         id_at[i] = tok - c * p.cache.page_size;
         id_page[i] = __ldg(p.table + pre.b * p.ld_table + c);

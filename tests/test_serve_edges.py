@@ -241,3 +241,24 @@ def test_prompt_items_longer_than_the_limit(f, shortest_limit, d, keys, rounds):
     a, b, c, cu_a, _ = prompt_case(5, [900, 77, 2000], [900, 77, 2000], 8, 2, d)
     check_prompt(f, a, b, c, cu_a, None)
     assert f.device_error() == 0
+
+
+@gpu
+def test_decode_of_the_longest_sequence(f):
+    """2^31 - 1 tokens (two pages in turn) beside 5: the sums of a lane have at most
+    2^31 / (2 * 148 * 4 warps * 8 lanes) additions, those of o half as many, each
+    within 2^-23, which bounds what they may be off by."""
+    d, page = 64, 1 << 16
+    kc, vc = randn(1, 2, page, 1, d).bfloat16(), randn(2, 2, page, 1, d).bfloat16()
+    table = (torch.arange(2 ** 31 // page + 1, device="cuda") % 2).int().repeat(2, 1)
+    lens = torch.tensor([2 ** 31 - 1, 5], dtype=torch.int32, device="cuda")
+    q = randn(3, 2, 4, d).bfloat16()
+    out, lse = f.paged_decode_attention(q, kc, vc, table, lens, return_lse=True)
+    k, v = kc.view(-1, 1, d), vc.view(-1, 1, d)
+    times = 2 ** 31 // (2 * page)
+    ref, a, l64, size = attend64(q[:1], k, v, d ** -0.5, torch.ones(1, 2 * page, dtype=torch.bool, device="cuda"))
+    off = 2 ** 31 / (2 * 148 * 4 * 8) * 2.0 ** -23
+    # (the token that is missing weighs less than 2^-31 e^size)
+    assert ((out[:1].double() - ref).abs() <= (2 * 2.0 ** -8 + off) * a + 2.0 ** -8 * ref.abs()).all()
+    assert ((lse[:1].double() - l64 - math.log(times)).abs() <= off + 2.0 ** -16 * (1 + size)).all()
+    check_attention(out[1:], lse[1:], *attend64(q[1:], k[:5], v[:5], d ** -0.5, torch.ones(1, 5, dtype=torch.bool, device="cuda")))
