@@ -380,7 +380,7 @@ int fp8gq_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_
   if (T < 0 || V < 1 || top_k < 0 || top_k > V) return FP8GQ_ERR_SHAPE;
   if (top_k > kMaxTop || (dtype != FP8GQ_DTYPE_BF16 && dtype != FP8GQ_DTYPE_F32)) return FP8GQ_ERR_UNSUPPORTED;
   if (T == 0) return FP8GQ_OK;
-  if (T > INT32_MAX / 16) return FP8GQ_ERR_UNSUPPORTED;
+  if (T > INT32_MAX / 16 || V > INT32_MAX - kLpThreads) return FP8GQ_ERR_UNSUPPORTED;     // (32-bit loops)
   if (!logits || (logprobs && !tokens) || (top_k > 0 && (!top_ids || !top_logprobs))) return FP8GQ_ERR_NULL_POINTER;
   if (T > 1 && ld < V) return FP8GQ_ERR_STRIDE;
   if (reinterpret_cast<uintptr_t>(logits) & (dtype == FP8GQ_DTYPE_BF16 ? 1u : 3u)) return FP8GQ_ERR_ALIGNMENT;

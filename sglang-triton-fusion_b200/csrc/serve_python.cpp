@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/fp8gq.h"
 
@@ -48,6 +49,13 @@ bool number(PyObject* o, double* v) {
   return !PyErr_Occurred();
 }
 
+// Whether the C entry points' int holds them.
+bool fits(std::initializer_list<int64_t> ns) {
+  for (int64_t n : ns)
+    if (n > INT32_MAX) return false;
+  return true;
+}
+
 // The cache of two tensors [pages, page_size, heads, D].
 bool paged_cache(PyObject* ko, PyObject* vo, PyObject* kso, PyObject* vso, int* device, fp8gq_paged_cache* c) {
   const at::Tensor *k = tensor(ko), *v = tensor(vo);
@@ -57,7 +65,7 @@ bool paged_cache(PyObject* ko, PyObject* vo, PyObject* kso, PyObject* vso, int* 
   if (k->scalar_type() != at::kBFloat16 && k->scalar_type() != at::kFloat8_e4m3fn) return false;
   const int d = k->get_device();
   if (*device < 0) *device = d;
-  if (d != *device || v->get_device() != d || k->stride(3) != 1 || v->stride(3) != 1) return false;
+  if (d != *device || v->get_device() != d || k->stride(3) != 1 || v->stride(3) != 1 || !fits({k->size(1)})) return false;
   double ks, vs;
   if (!number(kso, &ks) || !number(vso, &vs)) return false;
   *c = {k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1), k->stride(2), v->stride(0), v->stride(1), v->stride(2),
@@ -125,7 +133,7 @@ PyObject* qk_norm_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t t = qkv->size(0), d = k.size(3), hkv = k.size(2);
     if (d != 64 && d != 128) return not_here();
     const int64_t hq = qkv->size(1) / d - 2 * hkv;
-    if (qkv->size(1) % d || hkv < 1 || hq < 1 || hq % hkv) return not_here();
+    if (qkv->size(1) % d || hkv < 1 || hq < 1 || hq % hkv || !fits({t, hq, hkv})) return not_here();
     const at::Tensor *pos = vector(a[1], at::kLong, t, &dev), *slots = vector(a[2], at::kLong, t, &dev);
     const at::Tensor* cs = cuda_tensor(a[3], at::kFloat, 2, &dev);
     if (!pos || !slots || !cs || cs->size(1) != d || !cs->is_contiguous()) return not_here();
@@ -158,9 +166,10 @@ PyObject* paged_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!q || q->stride(2) != 1 || !paged_cache(a[1], a[2], a[6], a[7], &dev, &c)) return not_here();
     const at::Tensor& k = THPVariable_Unpack(a[1]);
     const int64_t b = q->size(0), hq = q->size(1), d = q->size(2), hkv = k.size(2);
-    if (k.size(3) != d || (d != 64 && d != 128) || hkv < 1 || hq < 1 || hq % hkv) return not_here();
+    if (k.size(3) != d || (d != 64 && d != 128) || hkv < 1 || hq < 1 || hq % hkv || !fits({b, hq, hkv})) return not_here();
     const at::Tensor *table = cuda_tensor(a[3], at::kInt, 2, &dev), *lens = vector(a[4], at::kInt, b, &dev);
-    if (!table || !lens || table->size(0) != b || (table->size(1) > 1 && table->stride(1) != 1)) return not_here();
+    if (!table || !lens || table->size(0) != b || (table->size(1) > 1 && table->stride(1) != 1) || !fits({table->size(1)}))
+      return not_here();
     double scale = 1.0 / std::sqrt(static_cast<double>(d));
     bool want_lse;
     if ((a[5] != Py_None && !number(a[5], &scale)) || !flag(a[8], &want_lse)) return not_here();
@@ -192,9 +201,10 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!q || !k || !v || q->stride(2) != 1 || k->stride(2) != 1 || v->stride(2) != 1 || k->sizes() != v->sizes())
       return not_here();
     const int64_t tq = q->size(0), hq = q->size(1), d = q->size(2), tk = k->size(0), hkv = k->size(1);
-    if (k->size(2) != d || (d != 64 && d != 128) || hkv < 1 || hq < 1 || hq % hkv) return not_here();
+    if (k->size(2) != d || (d != 64 && d != 128) || hkv < 1 || hq < 1 || hq % hkv || !fits({tq, tk, hq, hkv}))
+      return not_here();
     const at::Tensor* cq = cuda_tensor(a[3], at::kInt, 1, &dev);
-    if (!cq || cq->size(0) < 1 || !cq->is_contiguous()) return not_here();
+    if (!cq || cq->size(0) < 1 || !cq->is_contiguous() || !fits({cq->size(0)})) return not_here();
     const at::Tensor* ck = a[4] == Py_None ? cq : vector(a[4], at::kInt, cq->size(0), &dev);
     double scale = 1.0 / std::sqrt(static_cast<double>(d));
     bool causal, want_lse;
@@ -235,7 +245,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return not_here();
     int dev = x->get_device();
     const int64_t t = x->size(0), v = x->size(1);
-    if (v < 1 || (v > 1 && x->stride(1) != 1) || !PyLong_CheckExact(a[2])) return not_here();
+    if (v < 1 || (v > 1 && x->stride(1) != 1) || !fits({t, v}) || !PyLong_CheckExact(a[2])) return not_here();
     const long k = PyLong_AsLong(a[2]);
     if (k < 0 || k > 32 || k > v) return not_here();
     const at::Tensor* tok = nullptr;

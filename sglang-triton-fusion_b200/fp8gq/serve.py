@@ -81,6 +81,13 @@ def _check_device(*ts):
     return dev
 
 
+def _check_sizes(**sizes):
+    """The C entry points take 32-bit sizes (ctypes would cut larger ones)."""
+    for name, n in sizes.items():
+        if n > 2 ** 31 - 1:
+            raise ShapeError(f"at most 2^31 - 1 {name}, got {n}")
+
+
 def _check_cache(k, v, k_scale, v_scale):
     """Checks a paged cache; returns (its struct, Hkv, D)."""
     if k.dim() != 4 or k.shape != v.shape:
@@ -89,6 +96,7 @@ def _check_cache(k, v, k_scale, v_scale):
     if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
         raise TypeError(f"the cache must be bfloat16 or float8_e4m3fn, got {k.dtype} and {v.dtype}")
     pages, page, hkv, d = k.shape
+    _check_sizes(slots_per_page=page, heads=hkv)
     if d not in HEAD_DIMS:
         raise ShapeError(f"heads of {HEAD_DIMS} values, got {d}")
     ks, vs = k.stride(), v.stride()
@@ -145,6 +153,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise TypeError("qkv must be a 2-D bf16 tensor, contiguous along its last dimension")
     t, cols = qkv.shape
+    _check_sizes(tokens=t, columns=cols)
     hq = cols // d - 2 * hkv
     if cols % d or hq < 1 or hq % hkv:
         raise ShapeError(f"qkv has {cols} columns: expected (Hq + 2 * {hkv}) * {d} with Hq a multiple of {hkv}")
@@ -187,12 +196,14 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     dev = _check_device(q, k_cache, v_cache, page_table, lens, out)
     cache, hkv, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
     (b, hq, _), qs = _check_heads(q, "q", d)
+    _check_sizes(sequences=b, heads=hq)
     if hq % hkv:
         raise ShapeError(f"{hq} query heads are not a multiple of the cache's {hkv}")
     _check_vector(lens, "lens", b, torch.int32)
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b \
             or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ShapeError(f"page_table must be an int32 tensor [{b}, pages], contiguous along its last dimension")
+    _check_sizes(pages_per_sequence=page_table.shape[1])
     if out is None:
         out = torch.empty((b, hq, d), dtype=torch.bfloat16, device=dev)
         os = (hq * d, d)
@@ -234,6 +245,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     (tq, hq, d), qs = _check_heads(q, "q")
     (tk, hkv, _), ks = _check_heads(k, "k", d)
     vshape, vs = _check_heads(v, "v", d)
+    _check_sizes(tokens=max(tq, tk), heads=hq)
     if d not in HEAD_DIMS:
         raise ShapeError(f"heads of {HEAD_DIMS} values, got {d}")
     if vshape != k.shape or hkv < 1 or hq % hkv:
@@ -243,6 +255,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise ShapeError("cu_q must hold one offset more than there are sequences")
     n = cu_q.shape[0]
+    _check_sizes(offsets=n)
     _check_vector(cu_q, "cu_q", n, torch.int32)
     _check_vector(cu_k, "cu_k", n, torch.int32)
     if out is None:
@@ -290,6 +303,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     if logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2:
         raise TypeError("logits must be a 2-D bf16 or fp32 tensor")
     t, v = logits.shape
+    _check_sizes(rows=t, logits_per_row=v)
     if v < 1 or (v > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be contiguous along the vocabulary")
     if not 0 <= top_k <= min(MAX_TOP, v):

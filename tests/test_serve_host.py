@@ -98,3 +98,37 @@ def test_operands_on_two_devices_are_refused(lib, name):
             with pytest.raises(ValueError, match="one device"):
                 fp8gq.qk_norm_rope_append(*ts, **{kw: torch.ones(64, dtype=torch.bfloat16).as_subclass(on(1))})
     assert not lib.calls
+
+
+EMPTY = torch.empty          # (the fixture replaces it)
+
+
+def huge(*shape, dtype):
+    return EMPTY(*shape, dtype=dtype, device="meta").as_subclass(on(0))
+
+
+def test_sizes_past_32_bits_are_refused(lib):
+    """The entry points take 32-bit sizes; a larger one must not be cut to its low bits."""
+    n, b, i = 2 ** 32 + 5, torch.bfloat16, torch.int32
+    for x in (huge(n, 1, dtype=b), huge(1, n, dtype=torch.float32), huge(3, 2 ** 31, dtype=b)):
+        with pytest.raises(fp8gq.ShapeError, match="2.31"):
+            fp8gq.token_logprobs(x)
+    q, kc, vc, table, lens = [t.as_subclass(on(0)) for t in operands("paged_decode_attention")]
+    with pytest.raises(fp8gq.ShapeError, match="2.31"):
+        fp8gq.paged_decode_attention(q, kc, vc, huge(5, n, dtype=i), lens)
+    with pytest.raises(fp8gq.ShapeError, match="2.31"):
+        fp8gq.paged_decode_attention(q, huge(1, n, 2, 64, dtype=b), huge(1, n, 2, 64, dtype=b), table, lens)
+    big = huge(n, 2, 64, dtype=b)
+    with pytest.raises(fp8gq.ShapeError, match="2.31"):
+        fp8gq.prompt_attention(q, big, big, *[t.as_subclass(on(0)) for t in operands("prompt_attention")[3:]])
+    qkv, pos, slots, cs, kc, vc = [t.as_subclass(on(0)) for t in operands("qk_norm_rope_append")]
+    with pytest.raises(fp8gq.ShapeError, match="2.31"):
+        fp8gq.qk_norm_rope_append(huge(n, 8 * 64, dtype=b), huge(n, dtype=torch.int64), huge(n, dtype=torch.int64), cs, kc, vc)
+    assert not lib.calls
+
+
+def test_rows_that_32_bit_loops_cannot_walk_are_refused():
+    from fp8gq import _lib
+    a = 1 << 20
+    for v, want in ((2 ** 31 - 1, 8), (2 ** 31 - 100, 8)):
+        assert _lib.load().fp8gq_token_logprobs(a, v, 0, a, 1, v, a, a, a, a, 1, None) == want
