@@ -262,3 +262,60 @@ def test_decode_of_the_longest_sequence(f):
     assert ((out[:1].double() - ref).abs() <= (2 * 2.0 ** -8 + off) * a + 2.0 ** -8 * ref.abs()).all()
     assert ((lse[:1].double() - l64 - math.log(times)).abs() <= off + 2.0 ** -16 * (1 + size)).all()
     check_attention(out[1:], lse[1:], *attend64(q[1:], k[:5], v[:5], d ** -0.5, torch.ones(1, 5, dtype=torch.bool, device="cuda")))
+
+
+# ---------------------------------------------------------------- layouts --
+def heads_first(t):
+    """The same [tokens, heads, D] values laid out [heads, tokens, D]."""
+    return t.transpose(0, 1).contiguous().transpose(0, 1)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq, lk", [([70, 1, 200], [70, 1, 200]), ([9], [5000])])
+def test_prompt_heads_before_tokens(f, d, lq, lk):
+    q, k, v, cu_q, cu_k = prompt_case(31, lq, lk, 8, 2, d)
+    want, lse = check_prompt(f, q, k, v, cu_q, cu_k)
+    n = sum(lq)
+    out = heads_first(torch.zeros_like(q))
+    got, l2 = f.prompt_attention(heads_first(q), heads_first(k), heads_first(v), cu_q, cu_k, out=out, return_lse=True)
+    assert torch.equal(got[:n], want[:n]) and torch.equal(l2[:n], lse[:n])
+    assert torch.equal(f.prompt_attention(heads_first(q), k, heads_first(v), cu_q, cu_k)[:n], want[:n])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("order", [(0, 2, 1, 3), (2, 0, 1, 3), (1, 2, 0, 3)])
+def test_cache_layouts(f, dtype, order):
+    """Pages, slots and heads in other orders: append and decode as in the plain one."""
+    pages, page, hkv, d, hq = 7, 16, 2, 128, 8
+    k0, v0 = (randn(i, pages, page, hkv, d).to(dtype) for i in (1, 2))
+
+    def laid(t):
+        back = [order.index(i) for i in range(4)]
+        return t.view(torch.uint8).permute(*order).contiguous().permute(*back).view(dtype)
+
+    k1, v1 = laid(k0), laid(v0)
+    assert not k1.is_contiguous()
+    qkv, pos = randn(3, 5, (hq + 2 * hkv) * d).bfloat16(), torch.arange(5, device="cuda")
+    slots, cs = torch.tensor([0, 33, 111, -1, 64], device="cuda"), randn(4, 9, d)
+    a = f.qk_norm_rope_append(qkv, pos, slots, cs, k0, v0, k_scale=0.5, v_scale=0.25)
+    b = f.qk_norm_rope_append(qkv, pos, slots, cs, k1, v1, k_scale=0.5, v_scale=0.25)
+    bits = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
+    assert torch.equal(a, b) and torch.equal(bits(k0), bits(k1)) and torch.equal(bits(v0), bits(v1))
+    table = torch.tensor([[3, 0, 5], [6, 1, 2]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([41, 20], dtype=torch.int32, device="cuda")
+    q = heads_first(a[:2])
+    want = f.paged_decode_attention(a[:2], k0, v0, table, lens, return_lse=True)
+    got = f.paged_decode_attention(q, k1, v1, table, lens, out=heads_first(torch.zeros_like(a[:2])), return_lse=True)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+@gpu
+def test_heads_that_share_memory_are_refused(f):
+    """Broadcast heads (stride 0) have no place of their own: refused, not misread."""
+    q, k, v, cu, _ = prompt_case(32, [20], [20], 4, 1, 64, spare=0)
+    with pytest.raises(f.Fp8gqError):
+        f.prompt_attention(q, k.expand(20, 4, 64), v.expand(20, 4, 64), cu)
+    with pytest.raises(f.Fp8gqError):
+        f.prompt_attention(q, k, v, cu, out=torch.zeros(20, 1, 64, dtype=torch.bfloat16, device="cuda").expand(20, 4, 64))
