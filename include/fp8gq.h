@@ -600,7 +600,8 @@ int fp8gq_qk_norm_rope_append(const void *qkv, int64_t ldqkv, const int64_t *pos
  *   lens        int32 [B], the tokens a sequence has in the cache (the new one included)
  *   lse         fp32 [B, Hq] or NULL: log of the softmax's sum
  * A sequence of length 0 gives 0 (and lse -inf).  Scores, the softmax and the
- * sums are fp32.  A length past max_pages * page_size is cut there, a page
+ * sums are fp32; the weights meet v as bf16, with an e4m3 cache as f16 within 2^-40 of
+ * the largest.  A length past max_pages * page_size is cut there, a page
  * outside the cache counts as absent; both are recorded in the device error
  * word.  Slots past a sequence's length may hold anything, NaN included.
  * workspace as for the tile kernel: fp8gq_paged_decode_workspace_bytes bytes,
@@ -623,6 +624,7 @@ int fp8gq_paged_decode_attention(const void *q, int64_t q_token_stride, int64_t 
  *   causal  row i of a sequence sees keys j <= i + (k tokens - q tokens): its
  *           last row sees every key (a chunk of a prompt behind its prefix)
  *   lse     fp32 [Tq, Hq] or NULL
+ * Scores, the softmax and the sums are fp32; the weights meet v as bf16.
  * A row that sees no key gives 0 (and lse -inf).  Rows of out past cu_q[B] are
  * not written.  Values of other sequences never reach a row, NaN included; a
  * sequence's own k and v are taken to be finite (a masked v that is infinite

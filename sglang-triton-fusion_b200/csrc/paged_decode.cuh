@@ -9,7 +9,7 @@
 //
 // Work split: the tiles (4 warps x kTok tokens of one sequence and kv head) of
 // all sequences form one flat list, cut into equal contiguous ranges, one per
-// CTA, two or four CTAs per SM; the start of each (sequence, head) counts as
+// CTA, two CTAs per SM; the start of each (sequence, head) counts as
 // kDecItemCost tiles more.  The lengths are read on the device (a captured step
 // replays while they grow), so ragged batches and long single sequences
 // balance the same way.  A (sequence, head) that lies in several ranges leaves
@@ -17,17 +17,19 @@
 // order, so the result does not depend on who is last.
 //
 // Inside a CTA each warp runs alone: its lanes look up the pages of its own
-// kTok tokens and copy their rows of k and v (8 KB per step, kDecStages steps in
-// flight), and it computes on them with matrix instructions whose M side is the
+// kTok tokens and copy their rows of k and v (8 KB per step; while one of the
+// kDecStages is computed the other two are on their way), and it computes on them with matrix instructions whose M side is the
 // tokens (S^T = K Q^T, 16 x 8) and then the head's values (O^T = V^T P^T), so a
 // group of up to 8 query heads wastes nothing of K and V and no barrier stands
 // in the loop.  The copies are 16-byte cp.async: any page size and stride, and
 // one bulk copy per row was measured at 16 cycles each (8 x 32768 tokens, e4m3:
 // 235 us against 131 as the rest stood then).
 //
-// Measured, 32 query and 8 kv heads of 128: 64 x 4096 tokens 179 us (6.0 TB/s),
-// 48 ragged to 6000 69 us (5.7 TB/s), 8 x 32768 in e4m3 94 us (5.7 TB/s), 1 x 333
-// 8.1 us (the latency of one range and its join).
+// Measured in a CUDA graph, 32 query and 8 kv heads of 128: 64 x 4096 tokens 184 us
+// (5.8 TB/s), 48 ragged to 6000 71 us (5.5 TB/s), 8 x 32768 in e4m3 97 us (5.5
+// TB/s), 1 x 333 8.3 us (the latency of one range and its join).  More than 8 heads
+// a group, 10 x 1333 (16, 1, 128): 13.1 us in bf16 and in e4m3 (that build spills 208
+// bytes); 64 x 4096 (32, 2, 128): 59 us in bf16, 47 in e4m3, where conversions bound it.
 #pragma once
 
 #include "fp8gq_device.cuh"
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) paged_decode_kernel(con
   }
 
   // q as it lies: lane (g, t4) reads the values of head g that it will hold
-  constexpr int kRaw = kFp8 ? 2 * kKT : 2 * kKT;
+  constexpr int kRaw = 2 * kKT;
   uint32_t raw[kNT][kRaw];
   auto fetch_q = [&](const DecWalk& w) {
     const int hk = w.sub / p.blocks, hb = w.sub - hk * p.blocks;

@@ -44,7 +44,8 @@
 //
 // Measured, causal: 1 x 8192 (32 query and 8 kv heads of 128) 453 to 538 us from
 // one board to the next (1.0 to 1.2 PFLOP/s), 8 ragged to 700 38 us (fixed cost of
-// a call 7, of an item 2 to 4), 4 x 1024 ragged behind 5003 (16, 4, D = 64) 61 us.
+// a call 7, of an item 2 to 4), 4 x 1024 ragged behind 5003 (16, 4, D = 64) 60 to 72
+// us from one run to the next.
 //
 // Warps 0-3 and 4-7: softmax, output (one thread per row of tile 0, 1).  Warp 8:
 // TMA; it also clears the rows of the last v tile that lie past the sequence
@@ -672,7 +673,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_attention_kernel(const _
           m = mn;
         }
         const float mc = m == -INFINITY ? 0.0f : m * c;
-        // weights in bf16 (half an ulp each); l sums the unrounded
+        // weights in bf16, v's type, as the two operands of a product have one type:
+        // half an ulp each (more bits would take a second product); l sums the unrounded
         const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
         float2 sum[4];
 #pragma unroll

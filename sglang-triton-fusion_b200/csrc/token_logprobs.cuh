@@ -22,8 +22,9 @@
 // join in a fixed order and candidates are ranked by value and index, so
 // results do not depend on timing.
 //
-// Measured, 151936 logits a row: 2048 rows bf16 118 us (5.3 TB/s; MUFU 66 % and
-// issue 72 % busy), 37 rows fp32 13.5 us, 1 row bf16 8 us (latency).
+// Measured in a CUDA graph, 151936 logits a row: 2048 rows bf16 119 us (5.2 TB/s;
+// MUFU 66 % and issue 72 % busy), 37 rows fp32 13.1 to 13.6 us, 1 row bf16 8.2 to 8.8
+// us (latency).
 #pragma once
 
 #include "fp8gq_device.cuh"

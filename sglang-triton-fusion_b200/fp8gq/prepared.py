@@ -11,7 +11,8 @@ effect as the eager call it was prepared from.
 
 A plan holds raw pointers: it keeps the tensors it was prepared with alive,
 and must be prepared again when any of them is reallocated, or when
-set_static_weights / set_tm_options change.  Plans that share a workspace
+set_static_weights / set_tm_options change.  It is prepared before a graph capture,
+not within one.  Plans that share a workspace
 (all plans of one device and stream do) must not run concurrently.
 """
 from __future__ import annotations
