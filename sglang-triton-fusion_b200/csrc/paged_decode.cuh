@@ -18,12 +18,13 @@
 //
 // Inside a CTA each warp runs alone: its lanes look up the pages of its own
 // kTok tokens and copy their rows of k and v (8 KB per step; while one of the
-// kDecStages is computed the other two are on their way), and it computes on them with matrix instructions whose M side is the
-// tokens (S^T = K Q^T, 16 x 8) and then the head's values (O^T = V^T P^T), so a
-// group of up to 8 query heads wastes nothing of K and V and no barrier stands
-// in the loop.  The copies are 16-byte cp.async: any page size and stride, and
-// one bulk copy per row was measured at 16 cycles each (8 x 32768 tokens, e4m3:
-// 235 us against 131 as the rest stood then).
+// kDecStages is computed the other two are on their way), and it computes on
+// them with matrix instructions whose M side is the tokens (S^T = K Q^T, 16 x 8)
+// and then the head's values (O^T = V^T P^T), so a group of up to 8 query heads
+// wastes nothing of K and V and no barrier stands in the loop.  The copies are
+// 16-byte cp.async: any page size and stride, and one bulk copy per row was
+// measured at 16 cycles each (8 x 32768 tokens, e4m3: 235 us against 131 as the
+// rest stood then).
 //
 // Measured in a CUDA graph, 32 query and 8 kv heads of 128: 64 x 4096 tokens 184 us
 // (5.8 TB/s), 48 ragged to 6000 71 us (5.5 TB/s), 8 x 32768 in e4m3 97 us (5.5
